@@ -1,0 +1,1284 @@
+// Operators of a paged key/value cache for sm_100a: tables from request lengths, rotary positions, writing
+// new tokens into the pages, and the attention of one new token per request over them.  The interface, with
+// the formulas, is include/fa_paged_sm100.h.
+//
+// All of them are bound by memory or, for the small calls of a decoding step, by the latency of a launch:
+// none comes near the tensor pipe's rate (the attention does 4 flops per byte and query head of a group).
+//
+// Every kernel is launched chained to the kernel before it in the stream (programmatic stream serialization)
+// and executes griddepcontrol.wait before it first touches memory, so "the kernel before has finished" covers
+// all kernels before it.  Behind that wait nothing is read through the read-only path: no `__ldg`, no
+// `__restrict__` arguments (the compiler may move such loads ahead of the wait).
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstring>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "fa_paged_sm100.h"
+
+namespace fa_paged {
+
+// ------------------------------------------------------------------------------------------------
+// PTX wrappers
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// Lets the next kernel of the stream become resident / waits until the kernel before has finished.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// 16 bytes from global to shared memory; the rest of them is zero where `bytes` is less (0: nothing is read).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// Transposes the 8 x 8 matrix of 16-bit elements that the warp's registers hold.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+__device__ __forceinline__ long long load_int(const void* p, int is64, long long i) {
+    return is64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
+}
+
+// Inclusive prefix sum over the CTA (any multiple of 32 threads up to 1024); `scratch` holds 32 values.
+__device__ __forceinline__ long long block_scan(long long v, long long* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long n = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += n;
+    }
+    if (lane == 31) scratch[warp] = v;
+    __syncthreads();
+    long long before = 0;
+    for (int w = 0; w < warps; ++w)
+        if (w < warp) before += scratch[w];
+    __syncthreads();
+    return v + before;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Tables from request lengths
+// ------------------------------------------------------------------------------------------------
+// One CTA: a block-wide prefix sum over the requests (tokens, and pages needed), kept in shared memory; then
+// every thread takes tokens and finds each one's request by bisection.  What is read and written is a few
+// bytes per token: the time is that of a launch and of the few dependent reads.
+constexpr int kTableThreads = 1024;
+
+struct ExtendParams {
+    int* table;
+    long long table_stride;
+    const int* lens;
+    const int* new_lens;
+    const int* free_pages;
+    const int* free_head;
+    int* lens_out;
+    int* head_out;
+    long long* slots;
+    int* positions;
+    int* cu;
+    int batch, width, page_size, num_free;
+    long long num_tokens;
+};
+
+__device__ __forceinline__ long long div_up(long long a, long long b) { return (a + b - 1) / b; }
+
+__global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const ExtendParams p) {
+    extern __shared__ int s_table[];
+    int* s_cu = s_table;                       // batch + 1: first token of each request
+    int* s_len = s_cu + p.batch + 1;        // batch: length before
+    int* s_src = s_len + p.batch;           // batch: index of its first new page in the free list, -1: refused
+    __shared__ long long s_scan[32];
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    const int tid = threadIdx.x;
+    const int head = min(max(p.free_head[0], 0), p.num_free);
+    const long long avail = p.num_free - head;
+    long long tokens_before = 0, pages_before = 0;
+    int last_given = head;
+    for (int base = 0; base < p.batch; base += kTableThreads) {
+        const int b = base + tid;
+        const bool in = b < p.batch;
+        const long long len = in ? max(p.lens[b], 0) : 0, add = in ? max(p.new_lens[b], 0) : 0;
+        const long long have = div_up(len, p.page_size), want = div_up(len + add, p.page_size);
+        const bool fits = want <= p.width;
+        const long long need = fits ? want - have : 0;
+        const long long tokens = block_scan(add, s_scan) + tokens_before;
+        const long long pages = block_scan(need, s_scan) + pages_before;
+        const bool granted = fits && (need == 0 || pages <= avail);
+        if (in) {
+            s_cu[b + 1] = static_cast<int>(min(tokens, static_cast<long long>(INT_MAX)));
+            s_len[b] = static_cast<int>(len);
+            s_src[b] = granted ? head + static_cast<int>(pages - need) * (need > 0) : -1;
+            p.cu[b + 1] = s_cu[b + 1];
+            p.lens_out[b] = static_cast<int>(granted ? len + add : len);
+        }
+        // pages given so far: the prefix sum at the last request that was granted some
+        const int upto = in && granted && need > 0 ? head + static_cast<int>(pages) : head;
+        const int warp_most = __reduce_max_sync(0xffffffffu, upto);
+        if ((tid & 31) == 0) s_scan[tid >> 5] = warp_most;
+        __syncthreads();
+        for (int w = 0; w < kTableThreads / 32; ++w) last_given = max(last_given, static_cast<int>(s_scan[w]));
+        __syncthreads();
+        if (tid == kTableThreads - 1) {
+            s_scan[0] = tokens;
+            s_scan[1] = pages;
+        }
+        __syncthreads();
+        tokens_before = s_scan[0];
+        pages_before = s_scan[1];
+        __syncthreads();
+    }
+    if (tid == 0) {
+        s_cu[0] = 0;
+        p.cu[0] = 0;
+        p.head_out[0] = last_given;
+    }
+    __syncthreads();
+    // new pages: one warp per request
+    for (int b = tid >> 5; b < p.batch; b += kTableThreads / 32) {
+        if (s_src[b] < 0) continue;
+        const long long len = s_len[b], add = s_cu[b + 1] - s_cu[b];
+        const int have = static_cast<int>(div_up(len, p.page_size)), want = static_cast<int>(div_up(len + add, p.page_size));
+        int* row = p.table + b * p.table_stride;
+        for (int i = have + (tid & 31); i < want; i += 32) row[i] = p.free_pages[s_src[b] + i - have];
+    }
+    // slots and positions; a page that is new is read from the free list, not from the row just written
+    const long long total = s_cu[p.batch];
+    for (long long t = tid; t < p.num_tokens; t += kTableThreads) {
+        long long slot = -1;
+        int pos = 0;
+        if (t < total) {
+            int lo = 0, hi = p.batch;                    // s_cu[lo] <= t < s_cu[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (s_cu[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            pos = static_cast<int>(s_len[lo] + (t - s_cu[lo]));
+            if (s_src[lo] >= 0) {
+                const int have = static_cast<int>(div_up(s_len[lo], p.page_size)), at = pos / p.page_size;
+                const int page = at < have ? p.table[lo * p.table_stride + at] : p.free_pages[s_src[lo] + at - have];
+                slot = static_cast<long long>(page) * p.page_size + pos % p.page_size;
+            }
+        }
+        p.slots[t] = slot;
+        p.positions[t] = pos;
+    }
+}
+
+struct ShrinkParams {
+    const int* table;
+    long long table_stride;
+    int* lens;
+    const int* keep;
+    int* free_pages;
+    int* free_head;
+    int batch, width, page_size, num_free;
+};
+
+__global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const ShrinkParams p) {
+    extern __shared__ int s_table[];
+    int* s_from = s_table;                     // first page released
+    int* s_count = s_from + p.batch;        // pages released (0 for a refused request)
+    int* s_to = s_count + p.batch;          // where they go in the free list
+    __shared__ long long s_scan[32];
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    const int tid = threadIdx.x;
+    const int head = min(max(p.free_head[0], 0), p.num_free);
+    long long before = 0;
+    int lowest = head;
+    for (int base = 0; base < p.batch; base += kTableThreads) {
+        const int b = base + tid;
+        const bool in = b < p.batch;
+        const long long len = in ? max(p.lens[b], 0) : 0;
+        const long long keep = in ? min(static_cast<long long>(max(p.keep[b], 0)), len) : 0;
+        const long long most = p.width;
+        const long long from = min(div_up(keep, p.page_size), most), upto = min(div_up(len, p.page_size), most);
+        const long long count = upto - from;
+        const long long sum = block_scan(count, s_scan) + before;
+        const bool granted = count == 0 || sum <= head;
+        if (in) {
+            s_from[b] = static_cast<int>(from);
+            s_count[b] = granted ? static_cast<int>(count) : 0;
+            s_to[b] = granted ? head - static_cast<int>(sum) : 0;
+            if (granted) p.lens[b] = static_cast<int>(keep);
+        }
+        const int low = in && granted && count > 0 ? head - static_cast<int>(sum) : head;
+        const int warp_low = __reduce_min_sync(0xffffffffu, low);
+        if ((tid & 31) == 0) s_scan[tid >> 5] = warp_low;
+        __syncthreads();
+        for (int w = 0; w < kTableThreads / 32; ++w) lowest = min(lowest, static_cast<int>(s_scan[w]));
+        __syncthreads();
+        if (tid == kTableThreads - 1) s_scan[0] = sum;
+        __syncthreads();
+        before = s_scan[0];
+        __syncthreads();
+    }
+    for (int b = tid >> 5; b < p.batch; b += kTableThreads / 32) {
+        const int* row = p.table + b * p.table_stride + s_from[b];
+        for (int i = tid & 31; i < s_count[b]; i += 32) p.free_pages[s_to[b] + i] = row[i];
+    }
+    if (tid == 0) p.free_head[0] = lowest;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Rotary positions, and writing new tokens into the pages
+// ------------------------------------------------------------------------------------------------
+// One CTA per token: the angles of its position are worked out once, in shared memory, and serve all heads of
+// queries and keys.  A thread takes 8 elements and the 8 they are paired with (16-byte loads and stores).
+constexpr int kRotaryThreads = 128;
+
+struct Rows {                     // heads of one token: where they are read and where they go
+    const uint16_t* in;
+    uint16_t* out;
+    long long in_outer, in_head, in_token;     // element strides
+    long long out_outer, out_head, out_token;
+    int heads;
+    int turned;                   // 0: copied
+};
+
+struct RotaryParams {
+    Rows rows[3];                 // queries, keys, values
+    const double* freqs;          // NULL: nothing is turned
+    const void* positions;
+    long long position_outer;
+    int positions_64, rot, interleaved, head_dim;
+    float mscale, sign;
+    // tokens: grid.x = inner, grid.y = outer.  In the append form rows 1 and 2 go to the cache: out_token is
+    // the stride of a token in its page and out_outer that of a page.
+    const void* slots;            // NULL: not the append form
+    int slots_64, page_size;
+    long long num_slots;
+};
+
+template <bool BF16>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p) {
+    extern __shared__ float2 s_turn[];         // (cos, sin) * mscale of each pair
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    const int tid = threadIdx.x;
+    const long long token = blockIdx.x, outer = blockIdx.y;
+    const int pairs = p.rot / 2;
+    if (p.freqs != nullptr) {
+        const double pos = static_cast<double>(load_int(p.positions, p.positions_64, outer * p.position_outer + token));
+        for (int i = tid; i < pairs; i += kRotaryThreads) {
+            const double turns = pos * p.freqs[i] * 0.15915494309189533577;      // 1 / (2 pi)
+            float s, c;
+            sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+            s_turn[i] = make_float2(c * p.mscale, s * p.mscale * p.sign);
+        }
+        __syncthreads();
+    }
+    long long slot = 0;
+    if (p.slots != nullptr) slot = load_int(p.slots, p.slots_64, token);
+    const bool kept = slot >= 0 && (p.slots == nullptr || slot < p.num_slots);
+    const int chunks = p.head_dim / 8;
+    const int total = (p.rows[0].heads + p.rows[1].heads + p.rows[2].heads) * chunks;
+    for (int item = tid; item < total; item += kRotaryThreads) {
+        int head = item / chunks;
+        const int col = (item % chunks) * 8;
+        int which = 0;
+        while (head >= p.rows[which].heads) head -= p.rows[which++].heads;
+        const Rows& r = p.rows[which];
+        const uint16_t* in = r.in + outer * r.in_outer + token * r.in_token + head * r.in_head;
+        uint16_t* out;
+        if (p.slots != nullptr && which > 0) {
+            if (!kept) continue;
+            out = r.out + (slot / p.page_size) * r.out_outer + (slot % p.page_size) * r.out_token + head * r.out_head;
+        } else {
+            out = r.out + outer * r.out_outer + token * r.out_token + head * r.out_head;
+        }
+        uint4 v = *reinterpret_cast<const uint4*>(in + col);
+        if (p.freqs != nullptr && r.turned && col < p.rot) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 x = unpack2<BF16>(w[e]);
+                const int c0 = col + 2 * e;
+                if (p.interleaved) {
+                    if (c0 < p.rot) {
+                        const float2 t = s_turn[c0 / 2];
+                        w[e] = pack2<BF16>(x.x * t.x - x.y * t.y, x.y * t.x + x.x * t.y);
+                    }
+                } else {
+                    float y[2] = {x.x, x.y};
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int c = c0 + k;
+                        if (c >= p.rot) continue;
+                        const bool first = c < pairs;
+                        const int other = first ? c + pairs : c - pairs;
+                        const float o = unpack2<BF16>(in[other]).x;
+                        const float2 t = s_turn[first ? c : c - pairs];
+                        y[k] = first ? y[k] * t.x - o * t.y : y[k] * t.x + o * t.y;
+                    }
+                    w[e] = pack2<BF16>(y[0], y[1]);
+                }
+            }
+        }
+        *reinterpret_cast<uint4*>(out + col) = v;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Attention of one new token per request over the pages
+// ------------------------------------------------------------------------------------------------
+// Mathematics: one pass over the keys with a running maximum m, sum l and accumulator o per query head, in
+// fp32 and in powers of two: x = log2(e) * score, p = 2^(x - m), o = sum p v.  Parts of a key range are joined
+// by  o = sum_i 2^(m_i - m) o_i  and likewise l.
+//
+// Bound: memory.  A key of a KV head costs 4 * head_dim bytes and 4 * head_dim flops per query head of the
+// group, so even 32 heads a group stay far from the tensor pipe's balance (250 flops a byte).  What matters is
+// to keep enough loads in flight on every SM, whatever the lengths are.
+//
+// Work: the requests' key ranges, per KV head, are cut in tiles of kTile keys and laid one behind the other -
+// request, then KV head, then row block, then tile - and every CTA takes an equal, consecutive share of that
+// sequence.  The lengths are on the device only, so each CTA works out the sums itself.  A share may begin or
+// end inside a unit (one request and KV head): then it leaves a partial result (o, m, l) in the workspace and
+// paged_join_kernel joins the parts.  At most one such part at either end of a share.
+//
+// Inside a CTA four warps take the keys of a tile, kKeys each, and stream on their own: each has its own ring
+// of stages in shared memory, fills it by cp.async across tile, unit and request borders and never waits
+// for another warp before a unit ends; then the four results are joined through shared memory.
+//
+// Products: with few query rows the keys are the rows of the mma: S^T (16 keys x 8 heads) = K Q^T and
+// O^T (16 of d x 8 heads) += V^T P^T.  Eight heads to a tile waste half of what sixteen would, and the
+// accumulators are half as many.  K and V come through ldmatrix (V transposed); P^T moves from the accumulator
+// layout to the operand's by movmatrix.  mma.sync is enough here: at 8 heads a tile the tensor pipe is busy for
+// about a tenth of the time the loads take, and tcgen05's 128-row tiles would be filled with 8 rows or would
+// need P^T in shared memory.
+//
+// Precision: a weight p is the sum of two 16-bit numbers (hi + lo), two products instead of one; a single
+// 16-bit weight would add as much error as the rounding of the output.  Sums take the fp32 weight.
+constexpr int kWarps = 4;
+constexpr int kAttnThreads = kWarps * 32;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <int D>
+struct AttnCfg {
+    static constexpr int kKeys = 2048 / D;                 // keys of one warp's step: K and V are 4 KB each
+    static constexpr int kTile = kKeys * kWarps;
+    static constexpr int kStageBytes = kKeys * D * 2 * 2;
+    static constexpr int kStages = 3;
+    static constexpr int kRingBytes = kStageBytes * kStages * kWarps;
+    static constexpr int kJoinBytes = kWarps * 8 * D * 4;
+    static constexpr int kSmem = kRingBytes + kJoinBytes;
+};
+
+struct AttnParams {
+    const uint16_t* q;
+    uint16_t* out;
+    float* lse;
+    const uint16_t* k;
+    const uint16_t* v;
+    const int* table;
+    const int* lens;
+    const float* slopes;
+    long long q_batch, q_head, table_stride;
+    long long k_page, k_head, k_row, v_page, v_head, v_row;
+    int batch, heads, heads_k, group, row_blocks, width, page_size, num_pages, window;
+    float scale, cap;             // scale without log2(e)
+    // workspace
+    struct ShareInfo* info;       // one per CTA
+    float* parts;                 // two per CTA: rows * D of o, then rows (m, l)
+    long long part_floats;
+};
+
+// The unit in which a share begins, if it begins inside one.
+struct ShareInfo {
+    long long unit_begin, unit_end;       // its tiles in the sequence
+    long long total;                      // all tiles of the launch
+    int unit, inside, shares, pad;
+};
+
+struct Range {
+    int lo, hi;                   // visible keys [lo, hi)
+    int tile_lo, tile_hi;
+};
+__device__ __forceinline__ Range key_range(const AttnParams& p, int len, int tile) {
+    const int most = p.width * p.page_size;
+    Range r;
+    r.hi = min(max(len, 0), most);
+    r.lo = p.window > 0 ? max(0, r.hi - p.window) : 0;
+    r.tile_lo = r.lo / tile;
+    r.tile_hi = max(r.tile_lo + 1, (r.hi + tile - 1) / tile);     // a request without a key still takes one
+    return r;
+}
+
+// The share that tile `at` belongs to, of `shares` equal ones of `total` tiles: share c begins at
+// floor(c * total / shares).
+__device__ __forceinline__ int share_of(long long at, long long total, int shares) {
+    return static_cast<int>(((at + 1) * shares - 1) / total);
+}
+
+template <int D, bool BF16, int NT>
+__global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const AttnParams p) {
+    using C = AttnCfg<D>;
+    constexpr int MT = C::kKeys / 16, KK = D / 16, DT = D / 16, KEYS = C::kKeys, STAGES = C::kStages;
+    constexpr int ROWS = NT * 8;
+    extern __shared__ __align__(128) uint8_t s_ring[];
+    __shared__ long long s_scan[kWarps];
+    __shared__ long long s_start[2];
+    __shared__ float s_m[kWarps][8], s_l[kWarps][8];
+    struct Step { int b, unit, rel, last; uint32_t mask; int pad[3]; };
+    __shared__ Step s_step[kWarps][STAGES];
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per_request = p.heads_k * p.row_blocks;
+
+    // ---- my share
+    const int chunk = (p.batch + kAttnThreads - 1) / kAttnThreads;
+    const int b_lo = min(tid * chunk, p.batch), b_hi = min(b_lo + chunk, p.batch);
+    long long mine = 0;
+    for (int b = b_lo; b < b_hi; ++b) {
+        const Range r = key_range(p, p.lens[b], C::kTile);
+        mine += static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
+    }
+    const long long upto = block_scan(mine, s_scan);
+    if (tid == kAttnThreads - 1) s_start[0] = upto;
+    __syncthreads();
+    const long long total = s_start[0];
+    const int shares = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+    const int share = blockIdx.x;
+    if (share >= shares) {
+        if (tid == 0) p.info[share].inside = 0;
+        return;
+    }
+    const long long begin = share * total / shares, end = (share + 1) * total / shares;
+    __syncthreads();
+    if (begin >= upto - mine && begin < upto) {
+        long long at = upto - mine;
+        for (int b = b_lo; b < b_hi; ++b) {
+            const Range r = key_range(p, p.lens[b], C::kTile);
+            const long long n = static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
+            if (begin < at + n) {
+                s_start[0] = b;
+                s_start[1] = at;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+
+    // ---- the loader's place: request, unit within the request, tile
+    int lb = static_cast<int>(s_start[0]);
+    Range lr = key_range(p, p.lens[lb], C::kTile);
+    int lu, lt;
+    {
+        const long long off = begin - s_start[1];
+        const int tiles = lr.tile_hi - lr.tile_lo;
+        lu = static_cast<int>(off / tiles);
+        lt = lr.tile_lo + static_cast<int>(off % tiles);
+        if (tid == 0) {
+            ShareInfo info;
+            info.unit_begin = s_start[1] + static_cast<long long>(lu) * tiles;
+            info.unit_end = info.unit_begin + tiles;
+            info.total = total;
+            info.unit = lb * per_request + lu;
+            info.inside = info.unit_begin < begin;
+            info.shares = shares;
+            info.pad = 0;
+            p.info[share] = info;
+        }
+    }
+    const bool first_inside = lt > lr.tile_lo;       // the share begins inside a unit
+    long long to_load = end - begin;
+
+    const uint32_t ring_u = smem_u32(s_ring) + warp * (C::kStageBytes * STAGES);
+    float* join = reinterpret_cast<float*>(s_ring + C::kRingBytes);
+
+    auto load_step = [&](int stage) {
+        if (to_load > 0) {
+            const int key0 = lt * C::kTile + warp * KEYS;
+            // each lane looks up the page of one key
+            const int key = key0 + (lane % KEYS);
+            bool ok = key >= lr.lo && key < lr.hi;
+            long long ko = 0, vo = 0;
+            if (ok) {
+                const int at = key / p.page_size;
+                const int page = p.table[lb * p.table_stride + at], row = key - at * p.page_size;
+                ok = page >= 0 && page < p.num_pages;
+                if (ok) {
+                    ko = page * p.k_page + row * p.k_row;
+                    vo = page * p.v_page + row * p.v_row;
+                }
+            }
+            const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+            const int hk = lu / p.row_blocks;
+            const uint16_t* kb = p.k + hk * p.k_head;
+            const uint16_t* vb = p.v + hk * p.v_head;
+            const uint32_t dst = ring_u + stage * C::kStageBytes;
+            constexpr int CH = D / 8;                        // 16-byte chunks of a row
+            constexpr int RPI = 32 / CH;                     // rows of one instruction
+#pragma unroll
+            for (int i = 0; i < KEYS / RPI; ++i) {
+                const int row = i * RPI + lane / CH, col = lane % CH;
+                const long long kro = __shfl_sync(0xffffffffu, ko, row), vro = __shfl_sync(0xffffffffu, vo, row);
+                const uint32_t bytes = (mask >> row) & 1u ? 16u : 0u;
+                const uint32_t at = dst + row * (D * 2) + ((col ^ (row & 7)) << 4);
+                cp_async16(at, kb + kro + col * 8, bytes);
+                cp_async16(at + KEYS * D * 2, vb + vro + col * 8, bytes);
+            }
+            if (lane == 0) {
+                Step& st = s_step[warp][stage];
+                st.b = lb;
+                st.unit = lu;
+                st.rel = key0 - (lr.hi - 1);
+                st.mask = mask;
+                st.last = (to_load == 1 ? 1 : 0) | (lt + 1 == lr.tile_hi ? 2 : 0);
+            }
+            --to_load;
+            if (++lt == lr.tile_hi) {
+                if (++lu == per_request) {
+                    lu = 0;
+                    if (++lb < p.batch) lr = key_range(p, p.lens[lb], C::kTile);
+                }
+                lt = lr.tile_lo;
+            }
+        }
+        cp_async_commit();
+    };
+
+    for (int s = 0; s < STAGES - 1; ++s) load_step(s);
+
+    float o[DT][NT][4], m[NT][2], l[NT][2];
+    uint32_t qf[NT][KK][2];
+    float slope[NT][2];
+    const float scale2 = p.scale * kLog2e;
+    bool fresh = true;               // a unit begins
+    bool from_begin = !first_inside;
+    int stage = 0;
+    for (long long left = end - begin; left > 0; --left) {
+        __syncwarp();                // every lane has read the stage that is filled next
+        load_step(stage == 0 ? STAGES - 1 : stage - 1);
+        cp_async_wait<STAGES - 1>();
+        __syncwarp();
+        const Step st = s_step[warp][stage];
+        const int hk = st.unit / p.row_blocks, row0 = (st.unit % p.row_blocks) * ROWS;   // first query head in the group
+        if (fresh) {
+            fresh = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int r = row0 + n * 8 + lane / 4;
+                const uint16_t* qrow = p.q + st.b * p.q_batch + (static_cast<long long>(hk) * p.group + r) * p.q_head;
+#pragma unroll
+                for (int k = 0; k < KK; ++k) {
+                    const int c = k * 16 + (lane % 4) * 2;
+                    qf[n][k][0] = r < p.group ? *reinterpret_cast<const uint32_t*>(qrow + c) : 0u;
+                    qf[n][k][1] = r < p.group ? *reinterpret_cast<const uint32_t*>(qrow + c + 8) : 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    m[n][e] = -INFINITY;
+                    l[n][e] = 0.f;
+                    const int rr = row0 + n * 8 + (lane % 4) * 2 + e;
+                    slope[n][e] = p.slopes != nullptr && rr < p.group ? p.slopes[hk * p.group + rr] * kLog2e : 0.f;
+                }
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[t][n][e] = 0.f;
+            }
+        }
+        const uint32_t kaddr = ring_u + stage * C::kStageBytes, vaddr = kaddr + KEYS * D * 2;
+        // ---- S^T = K Q^T
+        float s[MT][NT][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][n][e] = 0.f;
+            const int row = t * 16 + (lane & 15);
+#pragma unroll
+            for (int k = 0; k < KK; ++k) {
+                uint32_t a[4];
+                ldmatrix_x4(a, kaddr + row * (D * 2) + (((k * 2 + (lane >> 4)) ^ (row & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816<BF16>(s[t][n], a, qf[n][k][0], qf[n][k][1]);
+            }
+        }
+        // ---- scores in powers of two
+        float top[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = t * 16 + lane / 4 + (e >> 1) * 8;
+                const bool seen = (st.mask >> key) & 1u;
+                const float back = static_cast<float>(st.rel + key);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float x;
+                    if (p.cap > 0.f) {
+                        // tanh(y) = 1 - 2 / (1 + e^(2y)): exact at both ends, absolute error of 2^-23 around 0
+                        const float y = s[t][n][e] * p.scale / p.cap;
+                        x = p.cap * kLog2e * (1.f - 2.f * rcp_approx(1.f + exp2_approx(2.f * kLog2e * y)));
+                    } else {
+                        x = s[t][n][e] * scale2;
+                    }
+                    x = fmaf(slope[n][e & 1], back, x);
+                    x = seen ? x : -INFINITY;
+                    s[t][n][e] = x;
+                    top[n][e & 1] = fmaxf(top[n][e & 1], x);
+                }
+            }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = top[n][e];
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                const float now = fmaxf(m[n][e], x);
+                const float ref = now == -INFINITY ? 0.f : now;
+                const float f = exp2_approx(m[n][e] - ref);
+                m[n][e] = now;
+                top[n][e] = ref;
+                l[n][e] *= f;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    o[t][n][e] *= f;
+                    o[t][n][e + 2] *= f;
+                }
+            }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float p0 = exp2_approx(s[t][n][2 * h] - top[n][0]);
+                    const float p1 = exp2_approx(s[t][n][2 * h + 1] - top[n][1]);
+                    l[n][0] += p0;
+                    l[n][1] += p1;
+                    const uint32_t w = pack2<BF16>(p0, p1);
+                    const float2 back = unpack2<BF16>(w);
+                    hi[n][h] = movmatrix(w);
+                    lo[n][h] = movmatrix(pack2<BF16>(p0 - back.x, p1 - back.y));
+                }
+            const int row = t * 16 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                uint32_t a[4];
+                ldmatrix_x4_trans(a, vaddr + row * (D * 2) + (((dt * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16816<BF16>(o[dt][n], a, hi[n][0], hi[n][1]);
+                    mma16816<BF16>(o[dt][n], a, lo[n][0], lo[n][1]);
+                }
+            }
+        }
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+
+        if (st.last != 0) {
+            // ---- the unit ends, or the share does: the four warps' results become one, eight heads at a time
+            const bool to_end = (st.last & 2) != 0;
+            float* part = p.parts + (2 * static_cast<long long>(share) + (from_begin ? 1 : 0)) * p.part_floats;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = l[n][e];
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    const int r = (lane % 4) * 2 + e;
+                    if (lane < 4) {
+                        s_m[warp][r] = m[n][e];
+                        s_l[warp][r] = x;
+                    }
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int d = t * 16 + h * 8 + lane / 4;
+                            join[(warp * 8 + r) * D + (d ^ ((lane % 4) * 8))] = o[t][n][e + 2 * h];
+                        }
+                }
+                __syncthreads();
+                for (int i = tid; i < 8 * D; i += kAttnThreads) {
+                    const int r = i / D, d = i % D, head = row0 + n * 8 + r;
+                    if (head >= p.group) break;
+                    float top4 = s_m[0][r];
+#pragma unroll
+                    for (int w = 1; w < kWarps; ++w) top4 = fmaxf(top4, s_m[w][r]);
+                    const float ref = top4 == -INFINITY ? 0.f : top4;
+                    float sum = 0.f, acc = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) {
+                        const float f = exp2_approx(s_m[w][r] - ref);
+                        sum = fmaf(f, s_l[w][r], sum);
+                        acc = fmaf(f, join[(w * 8 + r) * D + (d ^ ((r >> 1) * 8))], acc);
+                    }
+                    if (from_begin && to_end) {
+                        const long long h = static_cast<long long>(st.b) * p.heads + hk * p.group + head;
+                        const float v = sum == 0.f ? 0.f : acc / sum;
+                        p.out[h * D + d] = static_cast<uint16_t>(pack2<BF16>(v, 0.f));
+                        if (d == 0 && p.lse != nullptr)
+                            p.lse[h] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+                    } else {
+                        part[(n * 8 + r) * D + d] = acc;
+                        if (d == 0) {
+                            part[ROWS * D + 2 * (n * 8 + r)] = top4;
+                            part[ROWS * D + 2 * (n * 8 + r) + 1] = sum;
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+            fresh = true;
+            from_begin = true;
+        }
+    }
+    cp_async_wait<0>();
+}
+
+// Joins the parts of the units that several shares worked on.  CTA (x, y): the unit inside which share x + 1
+// begins, if that is the first border inside the unit, row y of it; the warps take the parts in turn.
+constexpr int kJoinThreads = 256;
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnParams p, int rows) {
+    __shared__ float s_o[kJoinThreads / 32][D];
+    __shared__ float s_m[kJoinThreads / 32], s_l[kJoinThreads / 32];
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    const int share = blockIdx.x + 1, row = blockIdx.y;
+    const ShareInfo info = p.info[share];
+    if (!info.inside) return;
+    const int first = share_of(info.unit_begin, info.total, info.shares);
+    if (share != first + 1) return;
+    const int last = share_of(info.unit_end - 1, info.total, info.shares);
+    const int per_request = p.heads_k * p.row_blocks;
+    const int b = info.unit / per_request, u = info.unit % per_request;
+    const int hk = u / p.row_blocks, head = (u % p.row_blocks) * rows + row;
+    if (head >= p.group) return;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int V = D / 32;
+    float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = 0.f;
+    for (int c = first + warp; c <= last; c += kJoinThreads / 32) {
+        const float* part = p.parts + (2 * static_cast<long long>(c) + (c == first ? 1 : 0)) * p.part_floats;
+        const float pm = part[rows * D + 2 * row], pl = part[rows * D + 2 * row + 1];
+        float x[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = part[row * D + i * 32 + lane];
+        const float now = fmaxf(m, pm), ref = now == -INFINITY ? 0.f : now;
+        const float f = exp2_approx(m - ref), g = exp2_approx(pm - ref);
+        m = now;
+        l = l * f + pl * g;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = o[i] * f + x[i] * g;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) s_o[warp][i * 32 + lane] = o[i];
+    if (lane == 0) {
+        s_m[warp] = m;
+        s_l[warp] = l;
+    }
+    __syncthreads();
+    if (tid >= D) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_m[w]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) {
+        const float f = exp2_approx(s_m[w] - ref);
+        sum = fmaf(f, s_l[w], sum);
+        acc = fmaf(f, s_o[w][tid], acc);
+    }
+    const long long h = static_cast<long long>(b) * p.heads + hk * p.group + head;
+    const float v = sum == 0.f ? 0.f : acc / sum;
+    p.out[h * D + tid] = static_cast<uint16_t>(pack2<BF16>(v, 0.f));
+    if (tid == 0 && p.lse != nullptr) p.lse[h] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------------------
+constexpr int kMaxDevices = 64;
+static std::atomic<unsigned long long> g_launches{0};
+static std::atomic<int> g_sm_count[kMaxDevices];       // 0: not asked yet, -1: not compute capability 10.x
+
+struct DeviceGuard {
+    int prev = -1;
+    bool switched = false;
+    cudaError_t err = cudaSuccess;
+    explicit DeviceGuard(int dev) {
+        err = cudaGetDevice(&prev);
+        if (err == cudaSuccess && prev != dev) {
+            err = cudaSetDevice(dev);
+            switched = err == cudaSuccess;
+        }
+    }
+    ~DeviceGuard() {
+        if (switched) cudaSetDevice(prev);
+    }
+};
+
+static int cuda_failed() {
+    cudaGetLastError();                                // do not leave the error for the caller's next call
+    return FA_PAGED_ERR_CUDA;
+}
+
+// SMs of the device, or a negative error code.
+static int sm_count(int device) {
+    int n = g_sm_count[device].load(std::memory_order_relaxed);
+    if (n == 0) {
+        int major = 0;
+        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess ||
+            cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+            return cuda_failed();
+        if (major != 10) n = -1;
+        g_sm_count[device].store(n, std::memory_order_relaxed);
+    }
+    return n > 0 ? n : FA_PAGED_ERR_ARCH;
+}
+
+template <typename Kern, typename... Args>
+static int launch_chained(Kern kern, dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return cuda_failed();
+    ++g_launches;
+    return FA_PAGED_OK;
+}
+
+// Dynamic shared memory above 48 KB has to be allowed once per kernel and device.
+template <typename Kern>
+static int allow_smem(Kern kern, int bytes, std::atomic<unsigned long long>& done, int device) {
+    const unsigned long long bit = 1ULL << device;
+    if (done.load(std::memory_order_acquire) & bit) return FA_PAGED_OK;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return cuda_failed();
+    done.fetch_or(bit, std::memory_order_release);
+    return FA_PAGED_OK;
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+static bool stride8(long long s) { return s >= 0 && s % 8 == 0; }
+
+static int check_device(int device) { return device >= 0 && device < kMaxDevices ? FA_PAGED_OK : FA_PAGED_ERR_SHAPE; }
+
+static int check_cache(const FaPagedCache& c) {
+    if (c.num_pages < 0 || c.heads_k <= 0 || c.page_size <= 0) return FA_PAGED_ERR_SHAPE;
+    if (c.head_dim != 64 && c.head_dim != 128) return FA_PAGED_ERR_HEAD_DIM;
+    if (c.num_pages > 0 && (c.k == nullptr || c.v == nullptr)) return FA_PAGED_ERR_NULL;
+    if (!aligned16(c.k) || !aligned16(c.v) || !stride8(c.k_page_stride) || !stride8(c.k_head_stride) ||
+        !stride8(c.k_row_stride) || !stride8(c.v_page_stride) || !stride8(c.v_head_stride) || !stride8(c.v_row_stride))
+        return FA_PAGED_ERR_ALIGN;
+    return FA_PAGED_OK;
+}
+
+static int check_rotary(const FaRotarySpec& r, int head_dim) {
+    if (r.freqs == nullptr || r.positions == nullptr) return FA_PAGED_ERR_NULL;
+    if (r.rot_dim < 2 || r.rot_dim > head_dim || r.rot_dim % 2 != 0) return FA_PAGED_ERR_ROTARY;
+    if (!std::isfinite(r.mscale)) return FA_PAGED_ERR_ROTARY;
+    return FA_PAGED_OK;
+}
+
+static void fill_rotary(RotaryParams* p, const FaRotarySpec& r) {
+    p->freqs = r.freqs;
+    p->positions = r.positions;
+    p->positions_64 = r.positions_64 != 0;
+    p->rot = r.rot_dim;
+    p->interleaved = r.interleaved != 0;
+    p->mscale = r.mscale;
+    p->sign = r.adjoint ? -1.f : 1.f;
+}
+
+static int launch_rotary(const RotaryParams& p, long long tokens, int outer, int dtype, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(outer));
+    const size_t smem = p.freqs != nullptr ? p.rot / 2 * sizeof(float2) : 0;
+    return dtype == FA_PAGED_BF16 ? launch_chained(rotary_kernel<true>, grid, kRotaryThreads, smem, stream, p)
+                                  : launch_chained(rotary_kernel<false>, grid, kRotaryThreads, smem, stream, p);
+}
+
+struct AttnPlan {
+    int grid, nt, row_blocks;
+    long long part_floats;
+    size_t info_bytes, bytes;
+};
+
+static int check_attention(const FaPagedAttentionArgs* a) {
+    if (a == nullptr) return FA_PAGED_ERR_NULL;
+    if (a->struct_size != sizeof(FaPagedAttentionArgs)) return FA_PAGED_ERR_ABI;
+    int rc = check_device(a->device);
+    if (rc != FA_PAGED_OK) return rc;
+    if (a->dtype != FA_PAGED_FP16 && a->dtype != FA_PAGED_BF16) return FA_PAGED_ERR_DTYPE;
+    rc = check_cache(a->cache);
+    if (rc != FA_PAGED_OK) return rc;
+    if (a->batch < 0 || a->heads < 0 || a->table_width < 0 || a->heads % a->cache.heads_k != 0 || a->table_stride < 0)
+        return FA_PAGED_ERR_SHAPE;
+    // key numbers are 32 bits, with room for the last tile; so are the units
+    if (static_cast<long long>(a->table_width) * a->cache.page_size > INT_MAX - 1024 ||
+        static_cast<long long>(a->batch) * a->heads > INT_MAX)
+        return FA_PAGED_ERR_SHAPE;
+    if (a->window < 0 || !std::isfinite(a->scale) || !std::isfinite(a->softcap) || a->scale < 0.f || a->softcap < 0.f)
+        return FA_PAGED_ERR_SCORE;
+    if (!aligned16(a->q) || !aligned16(a->out) || !stride8(a->q_batch_stride) || !stride8(a->q_head_stride))
+        return FA_PAGED_ERR_ALIGN;
+    return FA_PAGED_OK;
+}
+
+template <int D>
+static void make_attn_plan(const FaPagedAttentionArgs* a, int sms, AttnPlan* plan) {
+    const int group = a->heads / a->cache.heads_k;
+    plan->nt = group <= 8 ? 1 : 2;
+    plan->row_blocks = (group + plan->nt * 8 - 1) / (plan->nt * 8);
+    const long long tiles = (static_cast<long long>(a->table_width) * a->cache.page_size + AttnCfg<D>::kTile - 1) / AttnCfg<D>::kTile;
+    const long long most = static_cast<long long>(a->batch) * a->cache.heads_k * plan->row_blocks * (tiles > 0 ? tiles : 1);
+    const long long resident = 2LL * sms;
+    plan->grid = static_cast<int>(most < resident ? most : resident);
+    plan->part_floats = plan->nt * 8 * (D + 2);
+    plan->info_bytes = (plan->grid * sizeof(ShareInfo) + 255) / 256 * 256;
+    plan->bytes = plan->info_bytes + 2 * plan->grid * plan->part_floats * sizeof(float);
+}
+
+static int attn_plan(const FaPagedAttentionArgs* a, AttnPlan* plan) {
+    const int rc = check_attention(a);
+    if (rc != FA_PAGED_OK) return rc;
+    *plan = AttnPlan{};
+    if (a->batch == 0 || a->heads == 0) return FA_PAGED_OK;
+    const int sms = sm_count(a->device);
+    if (sms < 0) return sms;
+    if (a->cache.head_dim == 128) make_attn_plan<128>(a, sms, plan);
+    else make_attn_plan<64>(a, sms, plan);
+    return FA_PAGED_OK;
+}
+
+template <int D, bool BF16, int NT>
+static int launch_attention(const AttnParams& p, const AttnPlan& plan, int device, cudaStream_t stream) {
+    static std::atomic<unsigned long long> done{0};
+    int rc = allow_smem(paged_attention_kernel<D, BF16, NT>, AttnCfg<D>::kSmem, done, device);
+    if (rc != FA_PAGED_OK) return rc;
+    rc = launch_chained(paged_attention_kernel<D, BF16, NT>, dim3(plan.grid), kAttnThreads, AttnCfg<D>::kSmem, stream, p);
+    if (rc != FA_PAGED_OK || plan.grid < 2) return rc;
+    const int rows = p.group < NT * 8 ? p.group : NT * 8;
+    return launch_chained(paged_join_kernel<D, BF16>, dim3(plan.grid - 1, rows), kJoinThreads, 0, stream, p, NT * 8);
+}
+
+template <int D, bool BF16>
+static int dispatch_attention(const AttnParams& p, const AttnPlan& plan, int device, cudaStream_t stream) {
+    return plan.nt == 1 ? launch_attention<D, BF16, 1>(p, plan, device, stream)
+                        : launch_attention<D, BF16, 2>(p, plan, device, stream);
+}
+
+static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t bytes, cudaStream_t stream) {
+    AttnPlan plan;
+    const int rc = attn_plan(a, &plan);
+    if (rc != FA_PAGED_OK || plan.grid == 0) return rc;
+    if (a->q == nullptr || a->out == nullptr || a->lens == nullptr || (a->table_width > 0 && a->block_table == nullptr))
+        return FA_PAGED_ERR_NULL;
+    if (workspace == nullptr || bytes < plan.bytes || !aligned16(workspace)) return FA_PAGED_ERR_WORKSPACE;
+    DeviceGuard guard(a->device);
+    if (guard.err != cudaSuccess) return cuda_failed();
+    const FaPagedCache& c = a->cache;
+    AttnParams p = {};
+    p.q = static_cast<const uint16_t*>(a->q);
+    p.out = static_cast<uint16_t*>(a->out);
+    p.lse = a->lse;
+    p.k = static_cast<const uint16_t*>(c.k);
+    p.v = static_cast<const uint16_t*>(c.v);
+    p.table = a->block_table;
+    p.lens = a->lens;
+    p.slopes = a->slopes;
+    p.q_batch = a->q_batch_stride, p.q_head = a->q_head_stride, p.table_stride = a->table_stride;
+    p.k_page = c.k_page_stride, p.k_head = c.k_head_stride, p.k_row = c.k_row_stride;
+    p.v_page = c.v_page_stride, p.v_head = c.v_head_stride, p.v_row = c.v_row_stride;
+    p.batch = a->batch, p.heads = a->heads, p.heads_k = c.heads_k, p.group = a->heads / c.heads_k;
+    p.row_blocks = plan.row_blocks, p.width = a->table_width, p.page_size = c.page_size, p.num_pages = c.num_pages;
+    p.window = a->window, p.scale = a->scale, p.cap = a->softcap;
+    p.info = static_cast<ShareInfo*>(workspace);
+    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.info_bytes);
+    p.part_floats = plan.part_floats;
+    const bool bf16 = a->dtype == FA_PAGED_BF16;
+    if (c.head_dim == 128)
+        return bf16 ? dispatch_attention<128, true>(p, plan, a->device, stream)
+                    : dispatch_attention<128, false>(p, plan, a->device, stream);
+    return bf16 ? dispatch_attention<64, true>(p, plan, a->device, stream)
+                : dispatch_attention<64, false>(p, plan, a->device, stream);
+}
+
+static int rotary(const FaRotaryArgs* a, cudaStream_t stream) {
+    if (a == nullptr) return FA_PAGED_ERR_NULL;
+    if (a->struct_size != sizeof(FaRotaryArgs)) return FA_PAGED_ERR_ABI;
+    int rc = check_device(a->device);
+    if (rc != FA_PAGED_OK) return rc;
+    if (a->dtype != FA_PAGED_FP16 && a->dtype != FA_PAGED_BF16) return FA_PAGED_ERR_DTYPE;
+    if (a->batch < 0 || a->heads < 0 || a->heads_k < 0 || a->seqlen < 0 || a->position_batch_stride < 0)
+        return FA_PAGED_ERR_SHAPE;
+    if (a->head_dim != 64 && a->head_dim != 128) return FA_PAGED_ERR_HEAD_DIM;
+    if (a->batch > 65535 || static_cast<long long>(a->heads) + a->heads_k > (1 << 24)) return FA_PAGED_ERR_SHAPE;
+    if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->q_out) || !aligned16(a->k_out) || !stride8(a->q_batch_stride) ||
+        !stride8(a->q_head_stride) || !stride8(a->q_row_stride) || !stride8(a->k_batch_stride) || !stride8(a->k_head_stride) ||
+        !stride8(a->k_row_stride))
+        return FA_PAGED_ERR_ALIGN;
+    rc = check_rotary(a->rotary, a->head_dim);
+    const bool nothing = a->batch == 0 || a->seqlen == 0 || a->heads + a->heads_k == 0;
+    if (rc != FA_PAGED_OK && !(nothing && rc == FA_PAGED_ERR_NULL)) return rc;
+    if (nothing) return FA_PAGED_OK;
+    if ((a->heads > 0 && (a->q == nullptr || a->q_out == nullptr)) ||
+        (a->heads_k > 0 && (a->k == nullptr || a->k_out == nullptr)))
+        return FA_PAGED_ERR_NULL;
+    const int sms = sm_count(a->device);
+    if (sms < 0) return sms;
+    DeviceGuard guard(a->device);
+    if (guard.err != cudaSuccess) return cuda_failed();
+    RotaryParams p = {};
+    fill_rotary(&p, a->rotary);
+    const long long d = a->head_dim, plane = a->seqlen * d;
+    p.rows[0] = Rows{static_cast<const uint16_t*>(a->q), static_cast<uint16_t*>(a->q_out), a->q_batch_stride,
+                     a->q_head_stride, a->q_row_stride, a->heads * plane, plane, d, a->heads, 1};
+    p.rows[1] = Rows{static_cast<const uint16_t*>(a->k), static_cast<uint16_t*>(a->k_out), a->k_batch_stride,
+                     a->k_head_stride, a->k_row_stride, a->heads_k * plane, plane, d, a->heads_k, 1};
+    p.position_outer = a->position_batch_stride;
+    p.head_dim = a->head_dim;
+    return launch_rotary(p, a->seqlen, a->batch, a->dtype, stream);
+}
+
+static int append(const FaPagedAppendArgs* a, cudaStream_t stream) {
+    if (a == nullptr) return FA_PAGED_ERR_NULL;
+    if (a->struct_size != sizeof(FaPagedAppendArgs)) return FA_PAGED_ERR_ABI;
+    int rc = check_device(a->device);
+    if (rc != FA_PAGED_OK) return rc;
+    if (a->dtype != FA_PAGED_FP16 && a->dtype != FA_PAGED_BF16) return FA_PAGED_ERR_DTYPE;
+    rc = check_cache(a->cache);
+    if (rc != FA_PAGED_OK) return rc;
+    if (a->num_tokens < 0 || a->num_tokens > INT_MAX || a->heads < 0 ||
+        static_cast<long long>(a->heads) + 2LL * a->cache.heads_k > (1 << 24))
+        return FA_PAGED_ERR_SHAPE;
+    if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q_out) || !stride8(a->q_token_stride) ||
+        !stride8(a->q_head_stride) || !stride8(a->k_token_stride) || !stride8(a->k_head_stride) || !stride8(a->v_token_stride) ||
+        !stride8(a->v_head_stride))
+        return FA_PAGED_ERR_ALIGN;
+    const bool turned = a->rotary.freqs != nullptr;
+    if (turned) {
+        rc = check_rotary(a->rotary, a->cache.head_dim);
+        if (rc != FA_PAGED_OK && !(a->num_tokens == 0 && rc == FA_PAGED_ERR_NULL)) return rc;
+    }
+    if (a->num_tokens == 0) return FA_PAGED_OK;
+    if (a->k == nullptr || a->v == nullptr || a->slots == nullptr || (a->heads > 0 && (a->q == nullptr || a->q_out == nullptr)))
+        return FA_PAGED_ERR_NULL;
+    const int sms = sm_count(a->device);
+    if (sms < 0) return sms;
+    DeviceGuard guard(a->device);
+    if (guard.err != cudaSuccess) return cuda_failed();
+    const FaPagedCache& c = a->cache;
+    RotaryParams p = {};
+    if (turned) fill_rotary(&p, a->rotary);
+    const long long d = c.head_dim;
+    p.rows[0] = Rows{static_cast<const uint16_t*>(a->q), static_cast<uint16_t*>(a->q_out), 0, a->q_head_stride,
+                     a->q_token_stride, 0, d, a->heads * d, a->heads, 1};
+    p.rows[1] = Rows{static_cast<const uint16_t*>(a->k), static_cast<uint16_t*>(c.k), 0, a->k_head_stride,
+                     a->k_token_stride, c.k_page_stride, c.k_head_stride, c.k_row_stride, c.heads_k, 1};
+    p.rows[2] = Rows{static_cast<const uint16_t*>(a->v), static_cast<uint16_t*>(c.v), 0, a->v_head_stride,
+                     a->v_token_stride, c.v_page_stride, c.v_head_stride, c.v_row_stride, c.heads_k, 0};
+    p.head_dim = c.head_dim;
+    p.slots = a->slots;
+    p.slots_64 = a->slots_64 != 0;
+    p.page_size = c.page_size;
+    p.num_slots = static_cast<long long>(c.num_pages) * c.page_size;
+    return launch_rotary(p, a->num_tokens, 1, a->dtype, stream);
+}
+
+template <typename Args>
+static int check_table(const Args* a) {
+    if (a == nullptr) return FA_PAGED_ERR_NULL;
+    if (a->struct_size != sizeof(Args)) return FA_PAGED_ERR_ABI;
+    const int rc = check_device(a->device);
+    if (rc != FA_PAGED_OK) return rc;
+    if (a->batch < 0 || a->batch > FA_PAGED_MAX_REQUESTS || a->table_width < 0 || a->page_size <= 0 ||
+        a->num_free_pages < 0 || a->table_stride < 0 ||
+        static_cast<long long>(a->table_width) * a->page_size > INT_MAX)
+        return FA_PAGED_ERR_SHAPE;
+    if (a->free_head == nullptr || (a->batch > 0 && a->lens == nullptr) ||
+        (a->batch > 0 && a->table_width > 0 && a->block_table == nullptr) ||
+        (a->num_free_pages > 0 && a->free_pages == nullptr))
+        return FA_PAGED_ERR_NULL;
+    return FA_PAGED_OK;
+}
+
+static int extend(const FaPagedExtendArgs* a, cudaStream_t stream) {
+    const int rc = check_table(a);
+    if (rc != FA_PAGED_OK) return rc;
+    if (a->num_tokens < 0 || a->num_tokens > INT_MAX) return FA_PAGED_ERR_SHAPE;
+    if (a->cu == nullptr || a->head_out == nullptr || (a->batch > 0 && (a->new_lens == nullptr || a->lens_out == nullptr)) ||
+        (a->num_tokens > 0 && (a->slots == nullptr || a->positions == nullptr)))
+        return FA_PAGED_ERR_NULL;
+    const int sms = sm_count(a->device);
+    if (sms < 0) return sms;
+    DeviceGuard guard(a->device);
+    if (guard.err != cudaSuccess) return cuda_failed();
+    static std::atomic<unsigned long long> done{0};
+    const int most = (3 * FA_PAGED_MAX_REQUESTS + 1) * 4;
+    const int ok = allow_smem(paged_extend_kernel, most, done, a->device);
+    if (ok != FA_PAGED_OK) return ok;
+    ExtendParams p = {};
+    p.table = a->block_table, p.table_stride = a->table_stride, p.lens = a->lens, p.new_lens = a->new_lens;
+    p.free_pages = a->free_pages, p.free_head = a->free_head, p.lens_out = a->lens_out, p.head_out = a->head_out;
+    p.slots = reinterpret_cast<long long*>(a->slots), p.positions = a->positions, p.cu = a->cu;
+    p.batch = a->batch, p.width = a->table_width, p.page_size = a->page_size, p.num_free = a->num_free_pages;
+    p.num_tokens = a->num_tokens;
+    return launch_chained(paged_extend_kernel, dim3(1), kTableThreads, (3 * static_cast<size_t>(a->batch) + 1) * 4, stream, p);
+}
+
+static int shrink(const FaPagedShrinkArgs* a, cudaStream_t stream) {
+    const int rc = check_table(a);
+    if (rc != FA_PAGED_OK) return rc;
+    if (a->batch == 0) return FA_PAGED_OK;
+    if (a->keep_lens == nullptr) return FA_PAGED_ERR_NULL;
+    const int sms = sm_count(a->device);
+    if (sms < 0) return sms;
+    DeviceGuard guard(a->device);
+    if (guard.err != cudaSuccess) return cuda_failed();
+    static std::atomic<unsigned long long> done{0};
+    const int ok = allow_smem(paged_shrink_kernel, 3 * FA_PAGED_MAX_REQUESTS * 4, done, a->device);
+    if (ok != FA_PAGED_OK) return ok;
+    ShrinkParams p = {};
+    p.table = a->block_table, p.table_stride = a->table_stride, p.lens = a->lens, p.keep = a->keep_lens;
+    p.free_pages = a->free_pages, p.free_head = a->free_head;
+    p.batch = a->batch, p.width = a->table_width, p.page_size = a->page_size, p.num_free = a->num_free_pages;
+    return launch_chained(paged_shrink_kernel, dim3(1), kTableThreads, 3 * static_cast<size_t>(a->batch) * 4, stream, p);
+}
+
+}  // namespace fa_paged
+
+extern "C" {
+
+int fa_paged_extend_sm100(const FaPagedExtendArgs* args, void* stream) {
+    return fa_paged::extend(args, static_cast<cudaStream_t>(stream));
+}
+
+int fa_paged_shrink_sm100(const FaPagedShrinkArgs* args, void* stream) {
+    return fa_paged::shrink(args, static_cast<cudaStream_t>(stream));
+}
+
+int fa_rotary_sm100(const FaRotaryArgs* args, void* stream) {
+    return fa_paged::rotary(args, static_cast<cudaStream_t>(stream));
+}
+
+int fa_paged_append_sm100(const FaPagedAppendArgs* args, void* stream) {
+    return fa_paged::append(args, static_cast<cudaStream_t>(stream));
+}
+
+int fa_paged_attention_sm100_workspace_bytes(const FaPagedAttentionArgs* args, size_t* bytes) {
+    if (bytes == nullptr) return FA_PAGED_ERR_NULL;
+    fa_paged::AttnPlan plan;
+    const int rc = fa_paged::attn_plan(args, &plan);
+    if (rc == FA_PAGED_OK) *bytes = plan.bytes;
+    return rc;
+}
+
+int fa_paged_attention_sm100(const FaPagedAttentionArgs* args, void* workspace, size_t workspace_bytes, void* stream) {
+    return fa_paged::attention(args, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int fa_paged_sm100_abi_version(void) { return FA_PAGED_ABI_VERSION; }
+
+int fa_paged_sm100_launch_count(uint64_t* launches) {
+    if (launches == nullptr) return FA_PAGED_ERR_NULL;
+    *launches = fa_paged::g_launches.load();
+    return FA_PAGED_OK;
+}
+
+const char* fa_paged_sm100_strerror(int code) {
+    switch (code) {
+        case FA_PAGED_OK: return "ok";
+        case FA_PAGED_ERR_NULL: return "a required pointer is NULL";
+        case FA_PAGED_ERR_DTYPE: return "q, k, v and the cache must be float16 or bfloat16, of one type";
+        case FA_PAGED_ERR_SHAPE: return "bad shape: a size is negative or too large, or n_heads is not divisible by n_kv_heads";
+        case FA_PAGED_ERR_HEAD_DIM: return "Only head_dim=64 or head_dim=128 is supported";
+        case FA_PAGED_ERR_ALIGN: return "tensors must be 16-byte aligned, with strides that are multiples of 8 elements";
+        case FA_PAGED_ERR_WORKSPACE: return "workspace missing, misaligned or too small";
+        case FA_PAGED_ERR_ARCH: return "no kernel for this GPU: compute capability 10.x (sm_100a) required";
+        case FA_PAGED_ERR_CUDA: return "a CUDA call failed";
+        case FA_PAGED_ERR_ROTARY: return "rot_dim must be even, at least 2 and at most head_dim; mscale must be finite";
+        case FA_PAGED_ERR_SCORE: return "scale, softcap and window must be finite and not negative";
+        case FA_PAGED_ERR_ABI: return "struct_size does not match this library";
+        default: return "unknown error";
+    }
+}
+
+}  // extern "C"

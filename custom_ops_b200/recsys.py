@@ -9,8 +9,9 @@ reference ``recsys.py:165-202``), same lazy loading, the same loader checks afte
 ``__init__.py:910-934, 1069-1150``) and the same query API (``is_available``,
 ``load_error``, ``ensure_loaded``, ``groups``).
 
-Only the FA group exists here, only for sm_100a, and there is exactly one
-backend: hand-written CUDA.  ``backend="tilelang"`` and the automatic fallback of
+Of the reference's groups only the FA group exists here, only for sm_100a, and there is exactly one
+backend: hand-written CUDA.  A second group, ``PagedOps``, is this package's own: the operators of a
+paged key/value cache around that attention.  ``backend="tilelang"`` and the automatic fallback of
 the reference (``recsys.py:597-620``) are rejected, and a missing or unloadable
 native library raises instead of silently computing elsewhere.
 """
@@ -337,8 +338,84 @@ class FAOps(CustomOps):
                                lambda q, k, v, causal, window, valid_lens: torch.empty_like(q))
 
 
+class PagedOps(CustomOps):
+    """Paged key/value cache group: block tables, rotary positions, writing new tokens into the pages and
+    the attention of one new token per request over them; sm_100a kernels behind
+    ``include/fa_paged_sm100.h``.  The reference has no such group."""
+
+    namespace = "recsys_ops"
+    requires_cuda = True
+    so_name = "recsys_paged_kernel"
+    op_schemas = {
+        "paged_extend":
+            "paged_extend(Tensor(a!) block_table, Tensor seq_lens, Tensor new_lens, Tensor free_pages, "
+            "Tensor free_head, int page_size, int num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+        "paged_extend_":
+            "paged_extend_(Tensor(a!) block_table, Tensor(b!) seq_lens, Tensor new_lens, Tensor free_pages, "
+            "Tensor(c!) free_head, int page_size, int num_tokens) -> (Tensor, Tensor, Tensor)",
+        "paged_shrink_":
+            "paged_shrink_(Tensor block_table, Tensor(a!) seq_lens, Tensor keep_lens, Tensor(b!) free_pages, "
+            "Tensor(c!) free_head, int page_size) -> ()",
+        "rotary":
+            "rotary(Tensor q, Tensor k, Tensor positions, Tensor freqs, bool interleaved=False, float mscale=1.0, "
+            "bool adjoint=False) -> (Tensor, Tensor)",
+        "rotary_append":
+            "rotary_append(Tensor q, Tensor k, Tensor v, Tensor positions, Tensor slots, Tensor(a!) k_cache, "
+            "Tensor(b!) v_cache, Tensor freqs, bool interleaved=False, float mscale=1.0) -> Tensor",
+        "paged_append":
+            "paged_append(Tensor k, Tensor v, Tensor slots, Tensor(a!) k_cache, Tensor(b!) v_cache) -> ()",
+        "paged_attention":
+            "paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, "
+            "float? scale=None, int window=0, float softcap=0.0, Tensor? slopes=None) -> Tensor",
+        "paged_attention_lse":
+            "paged_attention_lse(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, "
+            "float? scale=None, int window=0, float softcap=0.0, Tensor? slopes=None) -> (Tensor, Tensor)",
+    }
+    required_ops = list(op_schemas)
+    fake_ops = list(op_schemas)
+
+    def get_sources(self) -> list:
+        return list(_build.PAGED_TORCH_SOURCES) + list(_build.PAGED_CABI_SOURCES)
+
+    def get_include_dirs(self) -> list:
+        return [_build.INCLUDE]
+
+    def build(self, *, force: bool = False, verbose: bool = False) -> str:
+        _build.build_paged_cabi(force=force, verbose=verbose)
+        return _build.build_paged_binding(force=force, verbose=verbose)
+
+    def prebuilt_path(self) -> str:
+        return _build.PAGED_TORCH_SO
+
+    def companion_libraries(self) -> list:
+        return [_build.PAGED_CABI_SO]
+
+    def register_fake_impls(self) -> None:
+        def tables(block_table, seq_lens, new_lens, free_pages, free_head, page_size, num_tokens):
+            return (seq_lens.new_empty((num_tokens,), dtype=torch.int64), seq_lens.new_empty((num_tokens,)),
+                    seq_lens.new_empty((seq_lens.shape[0] + 1,)))
+
+        def attention(q, k_cache, v_cache, block_table, seq_lens, scale=None, window=0, softcap=0.0, slopes=None):
+            return q.new_empty(q.shape)
+
+        def attention_lse(q, *args, **kwargs):
+            return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+        self.register_fake_for("paged_extend",
+                               lambda t, lens, new, free, head, ps, n: (torch.empty_like(lens), torch.empty_like(head))
+                               + tables(t, lens, new, free, head, ps, n))
+        self.register_fake_for("paged_extend_", tables)
+        self.register_fake_for("paged_shrink_", lambda *args: None)
+        self.register_fake_for("rotary", lambda q, k, positions, freqs, interleaved=False, mscale=1.0, adjoint=False:
+                               (q.new_empty(q.shape), k.new_empty(k.shape)))
+        self.register_fake_for("rotary_append", lambda q, *args, **kwargs: q.new_empty(q.shape))
+        self.register_fake_for("paged_append", lambda *args: None)
+        self.register_fake_for("paged_attention", attention)
+        self.register_fake_for("paged_attention_lse", attention_lse)
+
+
 class RecsysOps:
-    """Lazy facade over the operator groups (here: only "fa").
+    """Lazy facade over the operator groups: "fa", and this package's own "paged".
 
     The public surface -- ``configure``, ``disable_jit``, ``ensure_loaded``, ``load``, ``groups``,
     ``is_available``, ``load_error``, ``load_precompiled`` and the operators themselves -- is the
@@ -348,7 +425,12 @@ class RecsysOps:
     """
 
     _GROUP_CLASSES = {"fa": FAOps}
-    _OP_TO_GROUP = {"mha_fwd_with_mask": "fa", "mha_fwd_with_mask_lse": "fa", "mha_fwd_rule_mask": "fa"}
+    # Groups that the reference does not have: named like the others everywhere, but listed in ``groups`` and
+    # loaded by a bare ``ensure_loaded()`` only once somebody asked for them, so that a caller of the
+    # reference's groups sees and loads what it would see and load there.
+    _OWN_GROUP_CLASSES = {"paged": PagedOps}
+    _OP_TO_GROUP = {"mha_fwd_with_mask": "fa", "mha_fwd_with_mask_lse": "fa", "mha_fwd_rule_mask": "fa",
+                    **{name: "paged" for name in PagedOps.op_schemas}}
 
     def __init__(self, *, allow_jit: bool = True) -> None:
         self._allow_jit = bool(allow_jit)
@@ -376,9 +458,16 @@ class RecsysOps:
         return self.configure(allow_jit=False)
 
     # ---- the table of groups
+    def _group_class(self, name: str):
+        return self._GROUP_CLASSES.get(name) or self._OWN_GROUP_CLASSES.get(name)
+
+    def _listed(self) -> list:
+        return list(self._GROUP_CLASSES) + [n for n in self._OWN_GROUP_CLASSES if n in self._groups]
+
     def _validate_group(self, name: str) -> None:
-        if name not in self._GROUP_CLASSES:
-            raise ValueError(f"Unknown group {name!r}; available: {sorted(self._GROUP_CLASSES)}")
+        if self._group_class(name) is None:
+            raise ValueError(f"Unknown group {name!r}; available: "
+                             f"{sorted([*self._GROUP_CLASSES, *self._OWN_GROUP_CLASSES])}")
 
     def _peek(self, name: str):
         """The group's instance if somebody created it already, else None; never creates."""
@@ -391,7 +480,7 @@ class RecsysOps:
         with self._lock:
             inst = self._peek(name)
             if inst is None:
-                inst = self._groups[name] = self._GROUP_CLASSES[name](allow_jit=self._allow_jit)
+                inst = self._groups[name] = self._group_class(name)(allow_jit=self._allow_jit)
                 inst.load()
             return inst
 
@@ -406,15 +495,15 @@ class RecsysOps:
         with self._lock:
             inst = self._peek(group)
             if inst is None:
-                inst = self._GROUP_CLASSES[group](allow_jit=False)
+                inst = self._group_class(group)(allow_jit=False)
             inst.load_precompiled(path, metadata_path)
             self._groups[group] = inst
             return self
 
     def ensure_loaded(self, *names) -> "RecsysOps":
-        """Loads the named groups (all of them when none is named); unknown names are refused
+        """Loads the named groups (all that ``groups`` lists when none is named); unknown names are refused
         before anything is loaded."""
-        wanted = list(names) or list(self._GROUP_CLASSES)
+        wanted = list(names) or self._listed()
         with self._lock:
             for name in wanted:
                 self._validate_group(name)
@@ -428,7 +517,7 @@ class RecsysOps:
     @property
     def groups(self) -> dict:
         with self._lock:
-            return {name: self._state(name) for name in self._GROUP_CLASSES}
+            return {name: self._state(name) for name in self._listed()}
 
     def is_available(self, group: Optional[str] = None) -> bool:
         """One group: whether it is loaded and usable (loading it now unless building is off and
@@ -466,7 +555,7 @@ class RecsysOps:
         if group is None:
             raise AttributeError(
                 f"No op '{name}' in recsys_ops. Available ops: {sorted(self._OP_TO_GROUP)} "
-                f"(groups: {sorted(self._GROUP_CLASSES)})")
+                f"(groups: {sorted([*self._GROUP_CLASSES, *self._OWN_GROUP_CLASSES])})")
         return getattr(self._group(group), name)
 
     def __repr__(self) -> str:
@@ -503,3 +592,87 @@ class RecsysOps:
         merges: either may split long keys over the GPU, each in its own way.
         ``masks.rule_attention(..., single_pass=True)`` never does."""
         return self._dispatch(backend, "fa").mha_fwd_rule_mask(q, k, v, bool(causal), int(window), valid_lens)
+
+    # ---- the paged key/value cache (no counterpart in the reference)
+    def paged_extend(self, block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,
+                     free_pages: torch.Tensor, free_head: torch.Tensor, page_size: int, num_tokens: int,
+                     backend: Optional[str] = None):
+        """Gives each request the pages that its new tokens need, and says where the tokens go.
+
+        ``block_table`` int32 ``(B, W)``: the pages of each request, in order; new ones are written behind
+        those it has.  ``seq_lens``, ``new_lens`` int32 ``(B,)``: tokens held, tokens to add.  ``free_pages``
+        int32 ``(F,)`` is taken from index ``free_head`` (int32 ``(1,)``) on, in the order of the requests.
+        A request that the table has no columns for, or the list no pages, gets nothing; once the list has run
+        out, neither does any later request that needs a page.
+
+        Returns ``(seq_lens, free_head, slots, positions, cu)``: the new lengths (the old ones where refused)
+        and head, and for the ``num_tokens`` packed new tokens their slot (int64, ``page * page_size + row``;
+        -1 for a refused request and behind the last token), their position, and where each request's begin
+        (``cu``, ``(B + 1,)``).  Only ``block_table`` is written in place: the call may be repeated."""
+        return self._dispatch(backend, "paged").paged_extend(block_table, seq_lens, new_lens, free_pages, free_head,
+                                                             page_size, num_tokens)
+
+    def paged_extend_(self, block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,
+                      free_pages: torch.Tensor, free_head: torch.Tensor, page_size: int, num_tokens: int,
+                      backend: Optional[str] = None):
+        """``paged_extend`` that updates ``seq_lens`` and ``free_head`` in place - what a captured decoding
+        loop wants - and returns ``(slots, positions, cu)``."""
+        return self._dispatch(backend, "paged").paged_extend_(block_table, seq_lens, new_lens, free_pages, free_head,
+                                                              page_size, num_tokens)
+
+    def paged_shrink_(self, block_table: torch.Tensor, seq_lens: torch.Tensor, keep_lens: torch.Tensor,
+                      free_pages: torch.Tensor, free_head: torch.Tensor, page_size: int,
+                      backend: Optional[str] = None) -> None:
+        """Shortens every request to at most ``keep_lens`` tokens (0 releases it) and puts the pages behind that
+        back in front of ``free_head``.  ``seq_lens``, ``free_pages`` and ``free_head`` change in place."""
+        return self._dispatch(backend, "paged").paged_shrink_(block_table, seq_lens, keep_lens, free_pages, free_head,
+                                                              page_size)
+
+    def rotary(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,
+               interleaved: bool = False, mscale: float = 1.0, adjoint: bool = False, backend: Optional[str] = None):
+        """Rotary positions on q ``(B, H, S, d)`` and k ``(B, Hk, S, d)``, in the layout that the attention
+        takes: the inputs may be strided (a transposed projection), the results are contiguous.
+
+        ``positions`` int32 or int64 ``(S,)`` or ``(B, S)``; ``freqs`` float64, one angle per position and pair
+        (``paged.rotary_frequencies``): ``2 * len(freqs)`` elements of each head turn, in pairs ``(i, i + n)``
+        or, ``interleaved``, ``(2i, 2i + 1)``; the rest pass through.  Pairs are scaled by ``mscale``.  Nothing
+        here records gradients; ``adjoint`` turns the other way, which is the gradient with respect to q and k."""
+        return self._dispatch(backend, "paged").rotary(q, k, positions, freqs, interleaved, mscale, adjoint)
+
+    def rotary_append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                      slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, freqs: torch.Tensor,
+                      interleaved: bool = False, mscale: float = 1.0, backend: Optional[str] = None) -> torch.Tensor:
+        """Rotary positions on packed new tokens - q ``(T, H, d)``, k, v ``(T, Hk, d)``, strided views welcome -
+        and their keys and values written to ``slots`` of the caches ``(pages, Hk, page_size, d)``.  Returns the
+        turned q; a token whose slot is negative or behind the cache is not written."""
+        return self._dispatch(backend, "paged").rotary_append(q, k, v, positions, slots, k_cache, v_cache, freqs,
+                                                              interleaved, mscale)
+
+    def paged_append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
+                     v_cache: torch.Tensor, backend: Optional[str] = None) -> None:
+        """``rotary_append`` without the rotation, for models that have none."""
+        return self._dispatch(backend, "paged").paged_append(k, v, slots, k_cache, v_cache)
+
+    def paged_attention(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                        block_table: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
+                        window: int = 0, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                        backend: Optional[str] = None) -> torch.Tensor:
+        """Attention of one new token per request over its pages.
+
+        q ``(B, H, d)``, caches ``(pages, Hk, page_size, d)`` of q's dtype (any strides that keep the rows of
+        ``d`` whole), ``block_table`` int32 ``(B, W)``, ``seq_lens`` int32 ``(B,)`` counting the new token,
+        whose key and value are in the cache.  ``scale`` defaults to ``1 / sqrt(d)``; ``softcap > 0`` turns a
+        score x into ``softcap * tanh(x / softcap)``; ``slopes`` (fp32, one per head) add
+        ``slope * (key - newest key)``; ``window > 0`` hides all but the last ``window`` keys.
+        A request without a key gives 0."""
+        return self._dispatch(backend, "paged").paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale,
+                                                                window, softcap, slopes)
+
+    def paged_attention_lse(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            block_table: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
+                            window: int = 0, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                            backend: Optional[str] = None):
+        """``paged_attention`` that also returns each head's natural log-sum-exp, fp32 ``(B, H)``, ``-inf`` for a
+        request without a key: what a join with another part of the keys needs."""
+        return self._dispatch(backend, "paged").paged_attention_lse(q, k_cache, v_cache, block_table, seq_lens, scale,
+                                                                    window, softcap, slopes)

@@ -32,6 +32,13 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// 16 bytes; volatile, so that it stays where it is written: ahead of the work it is meant to overlap.
+__device__ __forceinline__ uint4 ld_v4(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // 16 bytes from global to shared memory; the rest of them is zero where `bytes` is less (0: nothing is read).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -100,7 +107,8 @@ __device__ __forceinline__ long long load_int(const void* p, int is64, long long
     return is64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
 }
 
-// Inclusive prefix sum over the CTA (any multiple of 32 threads up to 1024); `scratch` holds 32 values.
+// Inclusive prefix sum over the CTA (any multiple of 32 threads up to 1024); `scratch` holds 32 values and is
+// free again once the CTA has passed its next barrier.
 __device__ __forceinline__ long long block_scan(long long v, long long* scratch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
@@ -110,20 +118,38 @@ __device__ __forceinline__ long long block_scan(long long v, long long* scratch)
     }
     if (lane == 31) scratch[warp] = v;
     __syncthreads();
-    long long before = 0;
-    for (int w = 0; w < warps; ++w)
-        if (w < warp) before += scratch[w];
-    __syncthreads();
+    long long before = lane < warp && lane < warps ? scratch[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
     return v + before;
 }
 
 // ------------------------------------------------------------------------------------------------
 // Tables from request lengths
 // ------------------------------------------------------------------------------------------------
-// One CTA: a block-wide prefix sum over the requests (tokens, and pages needed), kept in shared memory; then
-// every thread takes tokens and finds each one's request by bisection.  What is read and written is a few
-// bytes per token: the time is that of a launch and of the few dependent reads.
-constexpr int kTableThreads = 1024;
+// A block-wide prefix sum over the requests (tokens, and pages needed), kept in shared memory; then every thread
+// takes four consecutive tokens at a time, finds the request of the first by bisection and walks on from there.
+// What is read and written is a few bytes per token: the time is that of a launch and of a chain of dependent
+// reads (lengths, free list, table).  Small calls are one CTA; from kTableTokens on it is a cluster of eight, each
+// of which works out the (cheap) sums for itself and takes an eighth of the tokens and pages.  A cluster and not
+// a grid, because lens and free_head may be updated in place: they are written behind a cluster barrier, when
+// every CTA has read them.
+constexpr int kTableThreads = 512;
+constexpr int kTableCluster = 8;
+constexpr long long kTableTokens = 4096;
+
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 struct ExtendParams {
     int* table;
@@ -145,17 +171,24 @@ __device__ __forceinline__ long long div_up(long long a, long long b) { return (
 
 __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const ExtendParams p) {
     extern __shared__ int s_table[];
-    int* s_cu = s_table;                       // batch + 1: first token of each request
+    int* s_cu = s_table;                    // batch + 1: first token of each request
     int* s_len = s_cu + p.batch + 1;        // batch: length before
     int* s_src = s_len + p.batch;           // batch: index of its first new page in the free list, -1: refused
-    __shared__ long long s_scan[32];
+    __shared__ long long s_scan[2][32];
+    __shared__ long long s_before[2];
+    __shared__ int s_head;
     pdl_launch_dependents();
-    pdl_wait_prior_grid();
     const int tid = threadIdx.x;
+    const unsigned rank = cluster_rank(), ranks = cluster_size();
+    pdl_wait_prior_grid();
     const int head = min(max(p.free_head[0], 0), p.num_free);
     const long long avail = p.num_free - head;
-    long long tokens_before = 0, pages_before = 0;
-    int last_given = head;
+    if (tid == 0) {
+        s_cu[0] = 0;
+        s_head = head;
+        s_before[0] = s_before[1] = 0;
+    }
+    __syncthreads();
     for (int base = 0; base < p.batch; base += kTableThreads) {
         const int b = base + tid;
         const bool in = b < p.batch;
@@ -163,67 +196,85 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
         const long long have = div_up(len, p.page_size), want = div_up(len + add, p.page_size);
         const bool fits = want <= p.width;
         const long long need = fits ? want - have : 0;
-        const long long tokens = block_scan(add, s_scan) + tokens_before;
-        const long long pages = block_scan(need, s_scan) + pages_before;
+        const long long tokens = s_before[0] + block_scan(add, s_scan[0]);
+        const long long pages = s_before[1] + block_scan(need, s_scan[1]);
         const bool granted = fits && (need == 0 || pages <= avail);
         if (in) {
             s_cu[b + 1] = static_cast<int>(min(tokens, static_cast<long long>(INT_MAX)));
             s_len[b] = static_cast<int>(len);
-            s_src[b] = granted ? head + static_cast<int>(pages - need) * (need > 0) : -1;
-            p.cu[b + 1] = s_cu[b + 1];
-            p.lens_out[b] = static_cast<int>(granted ? len + add : len);
+            s_src[b] = !granted ? -1 : need > 0 ? head + static_cast<int>(pages - need) : 0;
         }
-        // pages given so far: the prefix sum at the last request that was granted some
-        const int upto = in && granted && need > 0 ? head + static_cast<int>(pages) : head;
-        const int warp_most = __reduce_max_sync(0xffffffffu, upto);
-        if ((tid & 31) == 0) s_scan[tid >> 5] = warp_most;
-        __syncthreads();
-        for (int w = 0; w < kTableThreads / 32; ++w) last_given = max(last_given, static_cast<int>(s_scan[w]));
+        // pages are given to a first part of those that need some: the last prefix sum there is their number
+        const int given = __reduce_max_sync(0xffffffffu, in && granted && need > 0 ? head + static_cast<int>(pages) : 0);
+        if ((tid & 31) == 0 && given > 0) atomicMax(&s_head, given);
         __syncthreads();
         if (tid == kTableThreads - 1) {
-            s_scan[0] = tokens;
-            s_scan[1] = pages;
+            s_before[0] = tokens;
+            s_before[1] = pages;
         }
         __syncthreads();
-        tokens_before = s_scan[0];
-        pages_before = s_scan[1];
-        __syncthreads();
     }
-    if (tid == 0) {
-        s_cu[0] = 0;
-        p.cu[0] = 0;
-        p.head_out[0] = last_given;
-    }
-    __syncthreads();
+    cluster_arrive();                       // lens and free_head have been read
+    const unsigned page_size = p.page_size;
     // new pages: one warp per request
-    for (int b = tid >> 5; b < p.batch; b += kTableThreads / 32) {
+    const int warps = ranks * (kTableThreads / 32);
+    for (int b = rank * (kTableThreads / 32) + (tid >> 5); b < p.batch; b += warps) {
         if (s_src[b] < 0) continue;
-        const long long len = s_len[b], add = s_cu[b + 1] - s_cu[b];
-        const int have = static_cast<int>(div_up(len, p.page_size)), want = static_cast<int>(div_up(len + add, p.page_size));
+        const unsigned len = s_len[b], add = s_cu[b + 1] - s_cu[b];      // len + add: countable in 31 bits, or refused
+        const int have = (len + page_size - 1) / page_size, want = (len + add + page_size - 1) / page_size;
         int* row = p.table + b * p.table_stride;
         for (int i = have + (tid & 31); i < want; i += 32) row[i] = p.free_pages[s_src[b] + i - have];
     }
     // slots and positions; a page that is new is read from the free list, not from the row just written
     const long long total = s_cu[p.batch];
-    for (long long t = tid; t < p.num_tokens; t += kTableThreads) {
-        long long slot = -1;
-        int pos = 0;
-        if (t < total) {
-            int lo = 0, hi = p.batch;                    // s_cu[lo] <= t < s_cu[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (s_cu[mid] <= t) lo = mid;
+    const bool vec = ((reinterpret_cast<uintptr_t>(p.slots) | reinterpret_cast<uintptr_t>(p.positions)) & 15u) == 0;
+    for (long long t0 = 4 * (static_cast<long long>(rank) * kTableThreads + tid); t0 < p.num_tokens;
+         t0 += 4LL * ranks * kTableThreads) {
+        long long slot[4];
+        int pos[4];
+        int b = 0, hi = p.batch;                         // s_cu[b] <= t0 < s_cu[hi]
+        if (t0 < total)
+            while (hi - b > 1) {
+                const int mid = (b + hi) >> 1;
+                if (s_cu[mid] <= t0) b = mid;
                 else hi = mid;
             }
-            pos = static_cast<int>(s_len[lo] + (t - s_cu[lo]));
-            if (s_src[lo] >= 0) {
-                const int have = static_cast<int>(div_up(s_len[lo], p.page_size)), at = pos / p.page_size;
-                const int page = at < have ? p.table[lo * p.table_stride + at] : p.free_pages[s_src[lo] + at - have];
-                slot = static_cast<long long>(page) * p.page_size + pos % p.page_size;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const long long t = t0 + e;
+            slot[e] = -1;
+            pos[e] = 0;
+            if (t < total) {
+                while (s_cu[b + 1] <= t) ++b;
+                pos[e] = static_cast<int>(s_len[b] + (t - s_cu[b]));
+                if (s_src[b] >= 0) {
+                    const unsigned have = (s_len[b] + page_size - 1) / page_size, at = static_cast<unsigned>(pos[e]) / page_size;
+                    const int* from = at < have ? p.table + b * p.table_stride + at : p.free_pages + s_src[b] + (at - have);
+                    slot[e] = static_cast<long long>(*from) * page_size + (static_cast<unsigned>(pos[e]) - at * page_size);
+                }
             }
         }
-        p.slots[t] = slot;
-        p.positions[t] = pos;
+        if (vec && t0 + 4 <= p.num_tokens) {
+            *reinterpret_cast<longlong2*>(p.slots + t0) = make_longlong2(slot[0], slot[1]);
+            *reinterpret_cast<longlong2*>(p.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
+            *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (t0 + e < p.num_tokens) {
+                    p.slots[t0 + e] = slot[e];
+                    p.positions[t0 + e] = pos[e];
+                }
+        }
+    }
+    cluster_wait();
+    for (int b = rank * kTableThreads + tid; b < p.batch; b += ranks * kTableThreads) {
+        p.cu[b + 1] = s_cu[b + 1];
+        p.lens_out[b] = s_len[b] + (s_src[b] >= 0 ? s_cu[b + 1] - s_cu[b] : 0);
+    }
+    if (rank == 0 && tid == 0) {
+        p.cu[0] = 0;
+        p.head_out[0] = s_head;
     }
 }
 
@@ -239,16 +290,21 @@ struct ShrinkParams {
 
 __global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const ShrinkParams p) {
     extern __shared__ int s_table[];
-    int* s_from = s_table;                     // first page released
+    int* s_from = s_table;                  // first page released
     int* s_count = s_from + p.batch;        // pages released (0 for a refused request)
     int* s_to = s_count + p.batch;          // where they go in the free list
     __shared__ long long s_scan[32];
+    __shared__ long long s_before;
+    __shared__ int s_head;
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int tid = threadIdx.x;
     const int head = min(max(p.free_head[0], 0), p.num_free);
-    long long before = 0;
-    int lowest = head;
+    if (tid == 0) {
+        s_head = head;
+        s_before = 0;
+    }
+    __syncthreads();
     for (int base = 0; base < p.batch; base += kTableThreads) {
         const int b = base + tid;
         const bool in = b < p.batch;
@@ -257,7 +313,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const Shrin
         const long long most = p.width;
         const long long from = min(div_up(keep, p.page_size), most), upto = min(div_up(len, p.page_size), most);
         const long long count = upto - from;
-        const long long sum = block_scan(count, s_scan) + before;
+        const long long sum = s_before + block_scan(count, s_scan);
         const bool granted = count == 0 || sum <= head;
         if (in) {
             s_from[b] = static_cast<int>(from);
@@ -265,30 +321,27 @@ __global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const Shrin
             s_to[b] = granted ? head - static_cast<int>(sum) : 0;
             if (granted) p.lens[b] = static_cast<int>(keep);
         }
-        const int low = in && granted && count > 0 ? head - static_cast<int>(sum) : head;
-        const int warp_low = __reduce_min_sync(0xffffffffu, low);
-        if ((tid & 31) == 0) s_scan[tid >> 5] = warp_low;
+        const int low = __reduce_min_sync(0xffffffffu, in && granted && count > 0 ? head - static_cast<int>(sum) : INT_MAX);
+        if ((tid & 31) == 0) atomicMin(&s_head, low);
         __syncthreads();
-        for (int w = 0; w < kTableThreads / 32; ++w) lowest = min(lowest, static_cast<int>(s_scan[w]));
-        __syncthreads();
-        if (tid == kTableThreads - 1) s_scan[0] = sum;
-        __syncthreads();
-        before = s_scan[0];
+        if (tid == kTableThreads - 1) s_before = sum;
         __syncthreads();
     }
     for (int b = tid >> 5; b < p.batch; b += kTableThreads / 32) {
         const int* row = p.table + b * p.table_stride + s_from[b];
         for (int i = tid & 31; i < s_count[b]; i += 32) p.free_pages[s_to[b] + i] = row[i];
     }
-    if (tid == 0) p.free_head[0] = lowest;
+    if (tid == 0) p.free_head[0] = s_head;
 }
 
 // ------------------------------------------------------------------------------------------------
 // Rotary positions, and writing new tokens into the pages
 // ------------------------------------------------------------------------------------------------
 // One CTA per token: the angles of its position are worked out once, in shared memory, and serve all heads of
-// queries and keys.  A thread takes 8 elements and the 8 they are paired with (16-byte loads and stores).
+// queries and keys.  A thread takes 16 elements of a head, always the same ones, so the 8 pairs' cos and sin stay
+// in registers; the first kRotaryBatch heads' loads are in flight while the angles are worked out.
 constexpr int kRotaryThreads = 128;
+constexpr int kRotaryBatch = 3;
 
 struct Rows {                     // heads of one token: where they are read and where they go
     const uint16_t* in;
@@ -296,15 +349,14 @@ struct Rows {                     // heads of one token: where they are read and
     long long in_outer, in_head, in_token;     // element strides
     long long out_outer, out_head, out_token;
     int heads;
-    int turned;                   // 0: copied
 };
 
 struct RotaryParams {
-    Rows rows[3];                 // queries, keys, values
-    const double* freqs;          // NULL: nothing is turned
+    Rows rows[3];                 // queries and keys, which turn, and values, which do not
+    const double* freqs;
     const void* positions;
     long long position_outer;
-    int positions_64, rot, interleaved, head_dim;
+    int positions_64, rot;        // rot = 0: nothing turns
     float mscale, sign;
     // tokens: grid.x = inner, grid.y = outer.  In the append form rows 1 and 2 go to the cache: out_token is
     // the stride of a token in its page and out_outer that of a page.
@@ -313,15 +365,61 @@ struct RotaryParams {
     long long num_slots;
 };
 
-template <bool BF16>
+// How a head's elements are paired, and so which 16 a thread takes.
+enum Pairing {
+    kHalves,          // (i, i + rot / 2), rot a multiple of 16: 8 elements and the 8 they are paired with
+    kNeighbours,      // (2i, 2i + 1): 16 consecutive ones
+    kRaggedHalves     // (i, i + rot / 2) with any rot: 16 consecutive ones, the partners read one by one
+};
+
+template <int D, bool BF16, int PAIRING>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p) {
-    extern __shared__ float2 s_turn[];         // (cos, sin) * mscale of each pair
+    __shared__ __align__(16) float2 s_turn[D / 2 + 8];       // (cos, sin) * mscale of each pair
     pdl_launch_dependents();
-    pdl_wait_prior_grid();
     const int tid = threadIdx.x;
     const long long token = blockIdx.x, outer = blockIdx.y;
     const int pairs = p.rot / 2;
-    if (p.freqs != nullptr) {
+    constexpr int kParts = D / 16, kStep = kRotaryThreads / kParts;
+    const int part = tid % kParts;
+    const int col_a = PAIRING == kHalves ? (part * 16 < p.rot ? part * 8 : part * 16) : part * 16;
+    const int col_b = PAIRING == kHalves && part * 16 < p.rot ? col_a + pairs : col_a + 8;
+    const bool turned = part * 16 < p.rot;     // some of my elements turn
+    const int h0 = p.rows[0].heads, h1 = h0 + p.rows[1].heads, total = h1 + p.rows[2].heads;
+    auto source = [&](int head) {
+        const int which = head < h0 ? 0 : head < h1 ? 1 : 2;
+        const Rows& r = p.rows[which];
+        return r.in + outer * r.in_outer + token * r.in_token + (head - (which == 0 ? 0 : which == 1 ? h0 : h1)) * r.in_head;
+    };
+    pdl_wait_prior_grid();
+
+    uint4 a[kRotaryBatch], b[kRotaryBatch];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < kRotaryBatch; ++i) {
+            const int head = first + i * kStep;
+            if (head < total) {
+                const uint16_t* in = source(head);
+                a[i] = ld_v4(in + col_a);
+                b[i] = ld_v4(in + col_b);
+            }
+        }
+    };
+    load(tid / kParts);
+    long long page = 0, row = 0;
+    bool kept = true;
+    if (p.slots != nullptr) {
+        const long long slot = load_int(p.slots, p.slots_64, token);
+        kept = slot >= 0 && slot < p.num_slots;
+        if (slot <= UINT_MAX) {                // the usual case: no division in 64 bits
+            page = static_cast<unsigned>(slot) / static_cast<unsigned>(p.page_size);
+            row = static_cast<unsigned>(slot) - static_cast<unsigned>(page) * p.page_size;
+        } else {
+            page = slot / p.page_size;
+            row = slot - page * p.page_size;
+        }
+    }
+    float2 t[8];
+    if (p.rot > 0) {
         const double pos = static_cast<double>(load_int(p.positions, p.positions_64, outer * p.position_outer + token));
         for (int i = tid; i < pairs; i += kRotaryThreads) {
             const double turns = pos * p.freqs[i] * 0.15915494309189533577;      // 1 / (2 pi)
@@ -330,55 +428,70 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
             s_turn[i] = make_float2(c * p.mscale, s * p.mscale * p.sign);
         }
         __syncthreads();
-    }
-    long long slot = 0;
-    if (p.slots != nullptr) slot = load_int(p.slots, p.slots_64, token);
-    const bool kept = slot >= 0 && (p.slots == nullptr || slot < p.num_slots);
-    const int chunks = p.head_dim / 8;
-    const int total = (p.rows[0].heads + p.rows[1].heads + p.rows[2].heads) * chunks;
-    for (int item = tid; item < total; item += kRotaryThreads) {
-        int head = item / chunks;
-        const int col = (item % chunks) * 8;
-        int which = 0;
-        while (head >= p.rows[which].heads) head -= p.rows[which++].heads;
-        const Rows& r = p.rows[which];
-        const uint16_t* in = r.in + outer * r.in_outer + token * r.in_token + head * r.in_head;
-        uint16_t* out;
-        if (p.slots != nullptr && which > 0) {
-            if (!kept) continue;
-            out = r.out + (slot / p.page_size) * r.out_outer + (slot % p.page_size) * r.out_token + head * r.out_head;
-        } else {
-            out = r.out + outer * r.out_outer + token * r.out_token + head * r.out_head;
-        }
-        uint4 v = *reinterpret_cast<const uint4*>(in + col);
-        if (p.freqs != nullptr && r.turned && col < p.rot) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+        if (PAIRING != kRaggedHalves && turned)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 x = unpack2<BF16>(w[e]);
-                const int c0 = col + 2 * e;
-                if (p.interleaved) {
-                    if (c0 < p.rot) {
-                        const float2 t = s_turn[c0 / 2];
-                        w[e] = pack2<BF16>(x.x * t.x - x.y * t.y, x.y * t.x + x.x * t.y);
+            for (int i = 0; i < 4; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(&s_turn[part * 8 + 2 * i]);
+                t[2 * i] = make_float2(x.x, x.y);
+                t[2 * i + 1] = make_float2(x.z, x.w);
+            }
+    }
+    for (int first = tid / kParts; first < total; first += kRotaryBatch * kStep) {
+        if (first != tid / kParts) load(first);
+#pragma unroll
+        for (int i = 0; i < kRotaryBatch; ++i) {
+            const int head = first + i * kStep;
+            if (head >= total) break;
+            uint32_t* wa = reinterpret_cast<uint32_t*>(&a[i]);
+            uint32_t* wb = reinterpret_cast<uint32_t*>(&b[i]);
+            if (turned && head < h1) {
+                if constexpr (PAIRING == kHalves) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 x = unpack2<BF16>(wa[e]), y = unpack2<BF16>(wb[e]);
+                        const float2 t0 = t[2 * e], t1 = t[2 * e + 1];
+                        wa[e] = pack2<BF16>(x.x * t0.x - y.x * t0.y, x.y * t1.x - y.y * t1.y);
+                        wb[e] = pack2<BF16>(y.x * t0.x + x.x * t0.y, y.y * t1.x + x.y * t1.y);
+                    }
+                } else if constexpr (PAIRING == kNeighbours) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        uint32_t& w = e < 4 ? wa[e] : wb[e - 4];
+                        const float2 x = unpack2<BF16>(w);
+                        if (part * 8 + e < pairs) w = pack2<BF16>(x.x * t[e].x - x.y * t[e].y, x.y * t[e].x + x.x * t[e].y);
                     }
                 } else {
-                    float y[2] = {x.x, x.y};
+                    const uint16_t* in = source(head);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int c = c0 + k;
-                        if (c >= p.rot) continue;
-                        const bool first = c < pairs;
-                        const int other = first ? c + pairs : c - pairs;
-                        const float o = unpack2<BF16>(in[other]).x;
-                        const float2 t = s_turn[first ? c : c - pairs];
-                        y[k] = first ? y[k] * t.x - o * t.y : y[k] * t.x + o * t.y;
+                    for (int e = 0; e < 8; ++e) {
+                        uint32_t& w = e < 4 ? wa[e] : wb[e - 4];
+                        const float2 x = unpack2<BF16>(w);
+                        float y[2] = {x.x, x.y};
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int c = part * 16 + 2 * e + k;
+                            if (c >= p.rot) continue;
+                            const bool low = c < pairs;
+                            const float o = unpack2<BF16>(in[low ? c + pairs : c - pairs]).x;
+                            const float2 cs = s_turn[low ? c : c - pairs];
+                            y[k] = low ? y[k] * cs.x - o * cs.y : y[k] * cs.x + o * cs.y;
+                        }
+                        w = pack2<BF16>(y[0], y[1]);
                     }
-                    w[e] = pack2<BF16>(y[0], y[1]);
                 }
             }
+            const int which = head < h0 ? 0 : head < h1 ? 1 : 2;
+            const Rows& r = p.rows[which];
+            uint16_t* out = r.out + (head - (which == 0 ? 0 : which == 1 ? h0 : h1)) * r.out_head;
+            if (p.slots != nullptr && which > 0) {
+                if (!kept) continue;
+                out += page * r.out_outer + row * r.out_token;
+            } else {
+                out += outer * r.out_outer + token * r.out_token;
+            }
+            *reinterpret_cast<uint4*>(out + col_a) = a[i];
+            *reinterpret_cast<uint4*>(out + col_b) = b[i];
         }
-        *reinterpret_cast<uint4*>(out + col) = v;
     }
 }
 
@@ -910,20 +1023,27 @@ static int sm_count(int device) {
 }
 
 template <typename Kern, typename... Args>
-static int launch_chained(Kern kern, dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+static int launch_cluster(Kern kern, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return cuda_failed();
     ++g_launches;
     return FA_PAGED_OK;
+}
+template <typename Kern, typename... Args>
+static int launch_chained(Kern kern, dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+    return launch_cluster(kern, grid, threads, smem, 1, stream, args...);
 }
 
 // Dynamic shared memory above 48 KB has to be allowed once per kernel and device.
@@ -963,16 +1083,26 @@ static void fill_rotary(RotaryParams* p, const FaRotarySpec& r) {
     p->positions = r.positions;
     p->positions_64 = r.positions_64 != 0;
     p->rot = r.rot_dim;
-    p->interleaved = r.interleaved != 0;
     p->mscale = r.mscale;
     p->sign = r.adjoint ? -1.f : 1.f;
 }
 
-static int launch_rotary(const RotaryParams& p, long long tokens, int outer, int dtype, cudaStream_t stream) {
+template <int D, bool BF16>
+static int launch_rotary(const RotaryParams& p, bool interleaved, long long tokens, int outer, cudaStream_t stream) {
     const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(outer));
-    const size_t smem = p.freqs != nullptr ? p.rot / 2 * sizeof(float2) : 0;
-    return dtype == FA_PAGED_BF16 ? launch_chained(rotary_kernel<true>, grid, kRotaryThreads, smem, stream, p)
-                                  : launch_chained(rotary_kernel<false>, grid, kRotaryThreads, smem, stream, p);
+    if (interleaved) return launch_chained(rotary_kernel<D, BF16, kNeighbours>, grid, kRotaryThreads, 0, stream, p);
+    if (p.rot % 16 == 0) return launch_chained(rotary_kernel<D, BF16, kHalves>, grid, kRotaryThreads, 0, stream, p);
+    return launch_chained(rotary_kernel<D, BF16, kRaggedHalves>, grid, kRotaryThreads, 0, stream, p);
+}
+
+static int launch_rotary(const RotaryParams& p, bool interleaved, long long tokens, int outer, int head_dim, int dtype,
+                         cudaStream_t stream) {
+    const bool bf16 = dtype == FA_PAGED_BF16;
+    if (head_dim == 128)
+        return bf16 ? launch_rotary<128, true>(p, interleaved, tokens, outer, stream)
+                    : launch_rotary<128, false>(p, interleaved, tokens, outer, stream);
+    return bf16 ? launch_rotary<64, true>(p, interleaved, tokens, outer, stream)
+                : launch_rotary<64, false>(p, interleaved, tokens, outer, stream);
 }
 
 struct AttnPlan {
@@ -1110,12 +1240,11 @@ static int rotary(const FaRotaryArgs* a, cudaStream_t stream) {
     fill_rotary(&p, a->rotary);
     const long long d = a->head_dim, plane = a->seqlen * d;
     p.rows[0] = Rows{static_cast<const uint16_t*>(a->q), static_cast<uint16_t*>(a->q_out), a->q_batch_stride,
-                     a->q_head_stride, a->q_row_stride, a->heads * plane, plane, d, a->heads, 1};
+                     a->q_head_stride, a->q_row_stride, a->heads * plane, plane, d, a->heads};
     p.rows[1] = Rows{static_cast<const uint16_t*>(a->k), static_cast<uint16_t*>(a->k_out), a->k_batch_stride,
-                     a->k_head_stride, a->k_row_stride, a->heads_k * plane, plane, d, a->heads_k, 1};
+                     a->k_head_stride, a->k_row_stride, a->heads_k * plane, plane, d, a->heads_k};
     p.position_outer = a->position_batch_stride;
-    p.head_dim = a->head_dim;
-    return launch_rotary(p, a->seqlen, a->batch, a->dtype, stream);
+    return launch_rotary(p, a->rotary.interleaved != 0, a->seqlen, a->batch, a->head_dim, a->dtype, stream);
 }
 
 static int append(const FaPagedAppendArgs* a, cudaStream_t stream) {
@@ -1150,17 +1279,16 @@ static int append(const FaPagedAppendArgs* a, cudaStream_t stream) {
     if (turned) fill_rotary(&p, a->rotary);
     const long long d = c.head_dim;
     p.rows[0] = Rows{static_cast<const uint16_t*>(a->q), static_cast<uint16_t*>(a->q_out), 0, a->q_head_stride,
-                     a->q_token_stride, 0, d, a->heads * d, a->heads, 1};
+                     a->q_token_stride, 0, d, a->heads * d, a->heads};
     p.rows[1] = Rows{static_cast<const uint16_t*>(a->k), static_cast<uint16_t*>(c.k), 0, a->k_head_stride,
-                     a->k_token_stride, c.k_page_stride, c.k_head_stride, c.k_row_stride, c.heads_k, 1};
+                     a->k_token_stride, c.k_page_stride, c.k_head_stride, c.k_row_stride, c.heads_k};
     p.rows[2] = Rows{static_cast<const uint16_t*>(a->v), static_cast<uint16_t*>(c.v), 0, a->v_head_stride,
-                     a->v_token_stride, c.v_page_stride, c.v_head_stride, c.v_row_stride, c.heads_k, 0};
-    p.head_dim = c.head_dim;
+                     a->v_token_stride, c.v_page_stride, c.v_head_stride, c.v_row_stride, c.heads_k};
     p.slots = a->slots;
     p.slots_64 = a->slots_64 != 0;
     p.page_size = c.page_size;
     p.num_slots = static_cast<long long>(c.num_pages) * c.page_size;
-    return launch_rotary(p, a->num_tokens, 1, a->dtype, stream);
+    return launch_rotary(p, turned && a->rotary.interleaved != 0, a->num_tokens, 1, c.head_dim, a->dtype, stream);
 }
 
 template <typename Args>
@@ -1201,7 +1329,9 @@ static int extend(const FaPagedExtendArgs* a, cudaStream_t stream) {
     p.slots = reinterpret_cast<long long*>(a->slots), p.positions = a->positions, p.cu = a->cu;
     p.batch = a->batch, p.width = a->table_width, p.page_size = a->page_size, p.num_free = a->num_free_pages;
     p.num_tokens = a->num_tokens;
-    return launch_chained(paged_extend_kernel, dim3(1), kTableThreads, (3 * static_cast<size_t>(a->batch) + 1) * 4, stream, p);
+    const int ctas = a->num_tokens >= kTableTokens ? kTableCluster : 1;
+    return launch_cluster(paged_extend_kernel, dim3(ctas), kTableThreads, (3 * static_cast<size_t>(a->batch) + 1) * 4, ctas,
+                          stream, p);
 }
 
 static int shrink(const FaPagedShrinkArgs* a, cudaStream_t stream) {

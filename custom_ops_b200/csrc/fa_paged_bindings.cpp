@@ -11,6 +11,7 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -32,6 +33,11 @@ void check_rc(int rc, const char* op) { TORCH_CHECK(rc == FA_PAGED_OK, op, ": ",
 
 void* stream_of(const Tensor& t) {
     return static_cast<void*>(at::cuda::getCurrentCUDAStream(t.get_device()).stream());
+}
+
+// torch::empty without the dispatcher's way to it: these calls last a few microseconds.
+Tensor empty(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
+    return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
 }
 
 void check_cuda(const char* op, std::initializer_list<const Tensor*> tensors) {
@@ -134,8 +140,8 @@ Extended extend(const Tensor& block_table, const Tensor& seq_lens, const Tensor&
                 const Tensor& head_out, const char* op) {
     at::assert_no_internal_overlap(block_table);
     const int64_t B = block_table.size(0);
-    const auto opt = seq_lens.options();
-    Extended r{torch::empty({num_tokens}, opt.dtype(torch::kLong)), torch::empty({num_tokens}, opt), torch::empty({B + 1}, opt)};
+    Extended r{empty({num_tokens}, torch::kLong, seq_lens), empty({num_tokens}, torch::kInt, seq_lens),
+               empty({B + 1}, torch::kInt, seq_lens)};
     FaPagedExtendArgs a{};
     a.struct_size = sizeof(a);
     a.device = block_table.get_device();
@@ -171,7 +177,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_extend(const Tensor& bl
     check_table(block_table, seq_lens, new_lens, free_pages, free_head, page_size, op);
     check_num_tokens(num_tokens, op);
     const c10::cuda::CUDAGuard guard(block_table.device());
-    auto lens = torch::empty_like(seq_lens), head = torch::empty_like(free_head);
+    auto lens = empty({seq_lens.size(0)}, torch::kInt, seq_lens), head = empty({1}, torch::kInt, seq_lens);
     auto r = extend(block_table, seq_lens, new_lens, free_pages, free_head, page_size, num_tokens, lens, head, op);
     return {lens, head, r.slots, r.positions, r.cu};
 }
@@ -228,7 +234,7 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor
     TORCH_CHECK(S <= 1 || positions.stride(-1) == 1, op, ": the rows of positions must be contiguous");
     a.rotary = rotary_of(positions, freqs, interleaved, mscale, adjoint, d, op);
     const c10::cuda::CUDAGuard guard(q.device());
-    auto q_out = torch::empty({B, H, S, d}, q.options()), k_out = torch::empty({B, Hk, S, d}, k.options());
+    auto q_out = empty({B, H, S, d}, q.scalar_type(), q), k_out = empty({B, Hk, S, d}, q.scalar_type(), q);
     a.struct_size = sizeof(a);
     a.device = q.get_device();
     a.q = q.data_ptr();
@@ -283,7 +289,7 @@ Tensor rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Te
     check_list(positions, k.size(0), true, op, "positions");
     a.rotary = rotary_of(positions, freqs, interleaved, mscale, false, q.size(2), op);
     const c10::cuda::CUDAGuard guard(q.device());
-    auto out = torch::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+    auto out = empty({q.size(0), q.size(1), q.size(2)}, q.scalar_type(), q);
     a.q = q.data_ptr();
     a.q_out = out.data_ptr();
     a.q_token_stride = step(q, 0), a.q_head_stride = step(q, 1);
@@ -330,9 +336,9 @@ std::tuple<Tensor, Tensor> attention(const Tensor& q, const Tensor& k_cache, con
                     ": slopes must be a contiguous float32 tensor with one value per head");
     }
     const c10::cuda::CUDAGuard guard(q.device());
-    auto out = torch::empty({B, H, d}, q.options());
+    auto out = empty({B, H, d}, q.scalar_type(), q);
     Tensor lse;
-    if (want_lse) lse = torch::empty({B, H}, q.options().dtype(torch::kFloat));
+    if (want_lse) lse = empty({B, H}, torch::kFloat, q);
     a.struct_size = sizeof(a);
     a.device = q.get_device();
     a.q = q.data_ptr();
@@ -352,7 +358,7 @@ std::tuple<Tensor, Tensor> attention(const Tensor& q, const Tensor& k_cache, con
     size_t bytes = 0;
     check_rc(fa_paged_attention_sm100_workspace_bytes(&a, &bytes), op);
     Tensor ws;
-    if (bytes > 0) ws = torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(torch::kUInt8));
+    if (bytes > 0) ws = empty({static_cast<int64_t>(bytes)}, torch::kByte, q);
     check_rc(fa_paged_attention_sm100(&a, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q)), op);
     return {out, lse};
 }

@@ -167,7 +167,10 @@ struct ExtendParams {
     long long num_tokens;
 };
 
-__device__ __forceinline__ long long div_up(long long a, long long b) { return (a + b - 1) / b; }
+// Pages of so many tokens; no overflow, whatever is in the lengths.
+__device__ __forceinline__ unsigned pages_of(unsigned tokens, unsigned page_size) {
+    return tokens / page_size + (tokens % page_size != 0);
+}
 
 __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const ExtendParams p) {
     extern __shared__ int s_table[];
@@ -192,17 +195,17 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
     for (int base = 0; base < p.batch; base += kTableThreads) {
         const int b = base + tid;
         const bool in = b < p.batch;
-        const long long len = in ? max(p.lens[b], 0) : 0, add = in ? max(p.new_lens[b], 0) : 0;
-        const long long have = div_up(len, p.page_size), want = div_up(len + add, p.page_size);
-        const bool fits = want <= p.width;
-        const long long need = fits ? want - have : 0;
+        const unsigned len = in ? max(p.lens[b], 0) : 0, add = in ? max(p.new_lens[b], 0) : 0;
+        const unsigned have = pages_of(len, p.page_size), want = pages_of(len + add, p.page_size);
+        const bool fits = want <= static_cast<unsigned>(p.width);
+        const unsigned need = fits ? want - have : 0;
         const long long tokens = s_before[0] + block_scan(add, s_scan[0]);
         const long long pages = s_before[1] + block_scan(need, s_scan[1]);
         const bool granted = fits && (need == 0 || pages <= avail);
         if (in) {
             s_cu[b + 1] = static_cast<int>(min(tokens, static_cast<long long>(INT_MAX)));
             s_len[b] = static_cast<int>(len);
-            s_src[b] = !granted ? -1 : need > 0 ? head + static_cast<int>(pages - need) : 0;
+            s_src[b] = !granted ? -1 : need > 0 ? head + static_cast<int>(pages) - static_cast<int>(need) : 0;
         }
         // pages are given to a first part of those that need some: the last prefix sum there is their number
         const int given = __reduce_max_sync(0xffffffffu, in && granted && need > 0 ? head + static_cast<int>(pages) : 0);
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
     for (int b = rank * (kTableThreads / 32) + (tid >> 5); b < p.batch; b += warps) {
         if (s_src[b] < 0) continue;
         const unsigned len = s_len[b], add = s_cu[b + 1] - s_cu[b];      // len + add: countable in 31 bits, or refused
-        const int have = (len + page_size - 1) / page_size, want = (len + add + page_size - 1) / page_size;
+        const int have = pages_of(len, page_size), want = pages_of(len + add, page_size);
         int* row = p.table + b * p.table_stride;
         for (int i = have + (tid & 31); i < want; i += 32) row[i] = p.free_pages[s_src[b] + i - have];
     }
@@ -230,7 +233,8 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
     const bool vec = ((reinterpret_cast<uintptr_t>(p.slots) | reinterpret_cast<uintptr_t>(p.positions)) & 15u) == 0;
     for (long long t0 = 4 * (static_cast<long long>(rank) * kTableThreads + tid); t0 < p.num_tokens;
          t0 += 4LL * ranks * kTableThreads) {
-        long long slot[4];
+        const int* from[4];                              // where the page of each token is named
+        unsigned row[4];
         int pos[4];
         int b = 0, hi = p.batch;                         // s_cu[b] <= t0 < s_cu[hi]
         if (t0 < total)
@@ -242,18 +246,25 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const long long t = t0 + e;
-            slot[e] = -1;
+            from[e] = nullptr;
+            row[e] = 0;
             pos[e] = 0;
             if (t < total) {
                 while (s_cu[b + 1] <= t) ++b;
                 pos[e] = static_cast<int>(s_len[b] + (t - s_cu[b]));
                 if (s_src[b] >= 0) {
-                    const unsigned have = (s_len[b] + page_size - 1) / page_size, at = static_cast<unsigned>(pos[e]) / page_size;
-                    const int* from = at < have ? p.table + b * p.table_stride + at : p.free_pages + s_src[b] + (at - have);
-                    slot[e] = static_cast<long long>(*from) * page_size + (static_cast<unsigned>(pos[e]) - at * page_size);
+                    const unsigned have = pages_of(s_len[b], page_size), at = static_cast<unsigned>(pos[e]) / page_size;
+                    from[e] = at < have ? p.table + b * p.table_stride + at : p.free_pages + s_src[b] + (at - have);
+                    row[e] = static_cast<unsigned>(pos[e]) - at * page_size;
                 }
             }
         }
+        int page[4];
+        long long slot[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) page[e] = from[e] != nullptr ? *from[e] : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) slot[e] = from[e] != nullptr ? static_cast<long long>(page[e]) * page_size + row[e] : -1;
         if (vec && t0 + 4 <= p.num_tokens) {
             *reinterpret_cast<longlong2*>(p.slots + t0) = make_longlong2(slot[0], slot[1]);
             *reinterpret_cast<longlong2*>(p.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
@@ -308,11 +319,11 @@ __global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const Shrin
     for (int base = 0; base < p.batch; base += kTableThreads) {
         const int b = base + tid;
         const bool in = b < p.batch;
-        const long long len = in ? max(p.lens[b], 0) : 0;
-        const long long keep = in ? min(static_cast<long long>(max(p.keep[b], 0)), len) : 0;
-        const long long most = p.width;
-        const long long from = min(div_up(keep, p.page_size), most), upto = min(div_up(len, p.page_size), most);
-        const long long count = upto - from;
+        const unsigned len = in ? max(p.lens[b], 0) : 0;
+        const unsigned keep = in ? min(static_cast<unsigned>(max(p.keep[b], 0)), len) : 0;
+        const unsigned most = p.width;
+        const unsigned from = min(pages_of(keep, p.page_size), most), upto = min(pages_of(len, p.page_size), most);
+        const unsigned count = upto - from;
         const long long sum = s_before + block_scan(count, s_scan);
         const bool granted = count == 0 || sum <= head;
         if (in) {
@@ -337,11 +348,15 @@ __global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const Shrin
 // ------------------------------------------------------------------------------------------------
 // Rotary positions, and writing new tokens into the pages
 // ------------------------------------------------------------------------------------------------
-// One CTA per token: the angles of its position are worked out once, in shared memory, and serve all heads of
-// queries and keys.  A thread takes 16 elements of a head, always the same ones, so the 8 pairs' cos and sin stay
-// in registers; the first kRotaryBatch heads' loads are in flight while the angles are worked out.
+// A CTA takes 1, 2, 4 or 8 tokens: the angles of their positions are worked out once, in shared memory, and serve
+// all heads of queries and keys.  A thread takes 16 elements of a head, always the same ones of the same token, so
+// the 8 pairs' cos and sin stay in registers; the first kRotaryBatch heads' loads are in flight while the angles
+// are worked out.  Tokens per CTA: as many as keep a thread at kRotaryBatch heads at most, so that all of a CTA's
+// loads are in flight together - unless that leaves SMs without a CTA.
 constexpr int kRotaryThreads = 128;
-constexpr int kRotaryBatch = 3;
+constexpr int kRotaryBatch = 4;
+constexpr int kRotaryTokens = 8;
+constexpr int kRotaryWaves = 4;       // CTAs per SM that there have to be
 
 struct Rows {                     // heads of one token: where they are read and where they go
     const uint16_t* in;
@@ -358,7 +373,8 @@ struct RotaryParams {
     long long position_outer;
     int positions_64, rot;        // rot = 0: nothing turns
     float mscale, sign;
-    // tokens: grid.x = inner, grid.y = outer.  In the append form rows 1 and 2 go to the cache: out_token is
+    int tokens, per_cta;          // tokens of one outer index; tokens of a CTA
+    // grid.x: tokens, grid.y: outer.  In the append form rows 1 and 2 go to the cache: out_token is
     // the stride of a token in its page and out_outer that of a page.
     const void* slots;            // NULL: not the append form
     int slots_64, page_size;
@@ -374,17 +390,19 @@ enum Pairing {
 
 template <int D, bool BF16, int PAIRING>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p) {
-    __shared__ __align__(16) float2 s_turn[D / 2 + 8];       // (cos, sin) * mscale of each pair
+    __shared__ __align__(16) float2 s_turn[kRotaryTokens * D / 2];     // (cos, sin) * mscale of each pair
     pdl_launch_dependents();
     const int tid = threadIdx.x;
-    const long long token = blockIdx.x, outer = blockIdx.y;
+    constexpr int kParts = D / 16;
+    const int part = tid % kParts, mine = tid / kParts % p.per_cta, start = tid / kParts / p.per_cta;
+    const int step = kRotaryThreads / kParts / p.per_cta;
+    const long long outer = blockIdx.y, token0 = static_cast<long long>(blockIdx.x) * p.per_cta, token = token0 + mine;
     const int pairs = p.rot / 2;
-    constexpr int kParts = D / 16, kStep = kRotaryThreads / kParts;
-    const int part = tid % kParts;
+    const float2* turn = s_turn + mine * (D / 2);
     const int col_a = PAIRING == kHalves ? (part * 16 < p.rot ? part * 8 : part * 16) : part * 16;
     const int col_b = PAIRING == kHalves && part * 16 < p.rot ? col_a + pairs : col_a + 8;
     const bool turned = part * 16 < p.rot;     // some of my elements turn
-    const int h0 = p.rows[0].heads, h1 = h0 + p.rows[1].heads, total = h1 + p.rows[2].heads;
+    const int h0 = p.rows[0].heads, h1 = h0 + p.rows[1].heads, total = token < p.tokens ? h1 + p.rows[2].heads : 0;
     auto source = [&](int head) {
         const int which = head < h0 ? 0 : head < h1 ? 1 : 2;
         const Rows& r = p.rows[which];
@@ -396,7 +414,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
     auto load = [&](int first) {
 #pragma unroll
         for (int i = 0; i < kRotaryBatch; ++i) {
-            const int head = first + i * kStep;
+            const int head = first + i * step;
             if (head < total) {
                 const uint16_t* in = source(head);
                 a[i] = ld_v4(in + col_a);
@@ -404,10 +422,10 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
             }
         }
     };
-    load(tid / kParts);
+    load(start);
     long long page = 0, row = 0;
     bool kept = true;
-    if (p.slots != nullptr) {
+    if (p.slots != nullptr && token < p.tokens) {
         const long long slot = load_int(p.slots, p.slots_64, token);
         kept = slot >= 0 && slot < p.num_slots;
         if (slot <= UINT_MAX) {                // the usual case: no division in 64 bits
@@ -420,27 +438,30 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
     }
     float2 t[8];
     if (p.rot > 0) {
-        const double pos = static_cast<double>(load_int(p.positions, p.positions_64, outer * p.position_outer + token));
-        for (int i = tid; i < pairs; i += kRotaryThreads) {
+        constexpr int kLanes = kRotaryThreads / (D / 2);          // tokens worked on at a time, one pair a thread
+        const int i = tid % (D / 2);
+        for (int at = tid / (D / 2); at < p.per_cta; at += kLanes) {
+            if (i >= pairs || token0 + at >= p.tokens) continue;
+            const double pos = static_cast<double>(load_int(p.positions, p.positions_64, outer * p.position_outer + token0 + at));
             const double turns = pos * p.freqs[i] * 0.15915494309189533577;      // 1 / (2 pi)
             float s, c;
             sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
-            s_turn[i] = make_float2(c * p.mscale, s * p.mscale * p.sign);
+            s_turn[at * (D / 2) + i] = make_float2(c * p.mscale, s * p.mscale * p.sign);
         }
         __syncthreads();
         if (PAIRING != kRaggedHalves && turned)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float4 x = *reinterpret_cast<const float4*>(&s_turn[part * 8 + 2 * i]);
+                const float4 x = *reinterpret_cast<const float4*>(&turn[part * 8 + 2 * i]);
                 t[2 * i] = make_float2(x.x, x.y);
                 t[2 * i + 1] = make_float2(x.z, x.w);
             }
     }
-    for (int first = tid / kParts; first < total; first += kRotaryBatch * kStep) {
-        if (first != tid / kParts) load(first);
+    for (int first = start; first < total; first += kRotaryBatch * step) {
+        if (first != start) load(first);
 #pragma unroll
         for (int i = 0; i < kRotaryBatch; ++i) {
-            const int head = first + i * kStep;
+            const int head = first + i * step;
             if (head >= total) break;
             uint32_t* wa = reinterpret_cast<uint32_t*>(&a[i]);
             uint32_t* wb = reinterpret_cast<uint32_t*>(&b[i]);
@@ -473,7 +494,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
                             if (c >= p.rot) continue;
                             const bool low = c < pairs;
                             const float o = unpack2<BF16>(in[low ? c + pairs : c - pairs]).x;
-                            const float2 cs = s_turn[low ? c : c - pairs];
+                            const float2 cs = turn[low ? c : c - pairs];
                             y[k] = low ? y[k] * cs.x - o * cs.y : y[k] * cs.x + o * cs.y;
                         }
                         w = pack2<BF16>(y[0], y[1]);
@@ -530,16 +551,23 @@ constexpr int kAttnThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int D>
+template <int D, int NT>
 struct AttnCfg {
     static constexpr int kKeys = 2048 / D;                 // keys of one warp's step: K and V are 4 KB each
     static constexpr int kTile = kKeys * kWarps;
     static constexpr int kStageBytes = kKeys * D * 2 * 2;
-    static constexpr int kStages = 3;
+    // Stages and CTAs per SM, by what fits 227 KB; measured beside the launch (launch_attention).
+    static constexpr int kStages = NT > 2 || D == 64 ? 2 : 3;
+    static constexpr int kCtas = D == 64 && NT == 1 ? 3 : 2;
     static constexpr int kRingBytes = kStageBytes * kStages * kWarps;
     static constexpr int kJoinBytes = kWarps * 8 * D * 4;
+    // The query rows of a unit: in registers up to 16 heads; 32 would not fit beside the accumulators and stay in
+    // shared memory, in the buffer that joins the warps' results when the unit ends.
+    static constexpr bool kQueryInSmem = NT > 2;
     static constexpr int kSmem = kRingBytes + kJoinBytes;
+    static_assert(!kQueryInSmem || NT * 8 * D * 2 <= kJoinBytes, "the query rows fit the join buffer");
 };
+constexpr int attn_tile(int d) { return 2048 / d * kWarps; }
 
 struct AttnParams {
     const uint16_t* q;
@@ -553,7 +581,10 @@ struct AttnParams {
     long long q_batch, q_head, table_stride;
     long long k_page, k_head, k_row, v_page, v_head, v_row;
     int batch, heads, heads_k, group, row_blocks, width, page_size, num_pages, window;
-    float scale, cap;             // scale without log2(e)
+    unsigned page_mul, page_shift;      // key / page_size = key * page_mul >> page_shift, for keys below 2^31
+    // x, in powers of two, is s * scale2, or with a cap  cap2 * tanh(s * inner / 2),  inner = 2 log2(e) scale / cap:
+    // tanh(y) = 1 - 2 / (1 + 2^(2 log2(e) y))
+    float scale2, cap2, inner;
     // workspace
     struct ShareInfo* info;       // one per CTA
     float* parts;                 // two per CTA: rows * D of o, then rows (m, l)
@@ -571,25 +602,31 @@ struct Range {
     int lo, hi;                   // visible keys [lo, hi)
     int tile_lo, tile_hi;
 };
-__device__ __forceinline__ Range key_range(const AttnParams& p, int len, int tile) {
+template <int TILE>
+__device__ __forceinline__ Range key_range(const AttnParams& p, int len) {
     const int most = p.width * p.page_size;
     Range r;
     r.hi = min(max(len, 0), most);
     r.lo = p.window > 0 ? max(0, r.hi - p.window) : 0;
-    r.tile_lo = r.lo / tile;
-    r.tile_hi = max(r.tile_lo + 1, (r.hi + tile - 1) / tile);     // a request without a key still takes one
+    r.tile_lo = r.lo / TILE;
+    r.tile_hi = max(r.tile_lo + 1, (r.hi + TILE - 1) / TILE);     // a request without a key still takes one
     return r;
 }
 
-// The share that tile `at` belongs to, of `shares` equal ones of `total` tiles: share c begins at
-// floor(c * total / shares).
+// Share c of `shares` equal ones of `total` tiles begins at floor(c * total / shares).
+__device__ __forceinline__ long long share_begin(long long c, long long total, int shares) {
+    if (total < (1LL << 22)) return static_cast<unsigned>(c * total) / static_cast<unsigned>(shares);   // shares < 2^10
+    return c * total / shares;
+}
+// The share that tile `at` belongs to.
 __device__ __forceinline__ int share_of(long long at, long long total, int shares) {
+    if (total < (1LL << 22)) return static_cast<unsigned>((at + 1) * shares - 1) / static_cast<unsigned>(total);
     return static_cast<int>(((at + 1) * shares - 1) / total);
 }
 
-template <int D, bool BF16, int NT>
-__global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const AttnParams p) {
-    using C = AttnCfg<D>;
+template <int D, bool BF16, int NT, bool CAP>
+__global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_attention_kernel(const AttnParams p) {
+    using C = AttnCfg<D, NT>;
     constexpr int MT = C::kKeys / 16, KK = D / 16, DT = D / 16, KEYS = C::kKeys, STAGES = C::kStages;
     constexpr int ROWS = NT * 8;
     extern __shared__ __align__(128) uint8_t s_ring[];
@@ -608,7 +645,7 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
     const int b_lo = min(tid * chunk, p.batch), b_hi = min(b_lo + chunk, p.batch);
     long long mine = 0;
     for (int b = b_lo; b < b_hi; ++b) {
-        const Range r = key_range(p, p.lens[b], C::kTile);
+        const Range r = key_range<C::kTile>(p, p.lens[b]);
         mine += static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
     }
     const long long upto = block_scan(mine, s_scan);
@@ -621,12 +658,12 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
         if (tid == 0) p.info[share].inside = 0;
         return;
     }
-    const long long begin = share * total / shares, end = (share + 1) * total / shares;
+    const long long begin = share_begin(share, total, shares), end = share_begin(share + 1, total, shares);
     __syncthreads();
     if (begin >= upto - mine && begin < upto) {
         long long at = upto - mine;
         for (int b = b_lo; b < b_hi; ++b) {
-            const Range r = key_range(p, p.lens[b], C::kTile);
+            const Range r = key_range<C::kTile>(p, p.lens[b]);
             const long long n = static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
             if (begin < at + n) {
                 s_start[0] = b;
@@ -640,13 +677,13 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
 
     // ---- the loader's place: request, unit within the request, tile
     int lb = static_cast<int>(s_start[0]);
-    Range lr = key_range(p, p.lens[lb], C::kTile);
+    Range lr = key_range<C::kTile>(p, p.lens[lb]);
     int lu, lt;
     {
-        const long long off = begin - s_start[1];
-        const int tiles = lr.tile_hi - lr.tile_lo;
-        lu = static_cast<int>(off / tiles);
-        lt = lr.tile_lo + static_cast<int>(off % tiles);
+        const unsigned off = static_cast<unsigned>(begin - s_start[1]);     // below tiles * per_request: 31 bits, checked
+        const unsigned tiles = lr.tile_hi - lr.tile_lo;
+        lu = off / tiles;
+        lt = lr.tile_lo + off % tiles;
         if (tid == 0) {
             ShareInfo info;
             info.unit_begin = s_start[1] + static_cast<long long>(lu) * tiles;
@@ -660,58 +697,87 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
         }
     }
     const bool first_inside = lt > lr.tile_lo;       // the share begins inside a unit
-    long long to_load = end - begin;
+    int to_load = static_cast<int>(end - begin);
 
     const uint32_t ring_u = smem_u32(s_ring) + warp * (C::kStageBytes * STAGES);
     float* join = reinterpret_cast<float*>(s_ring + C::kRingBytes);
+    const uint32_t join_u = smem_u32(join);
+
+    constexpr int CH = D / 8;                        // 16-byte chunks of a row
+    constexpr int RPI = 32 / CH;                     // rows that one instruction of the warp loads
+    const bool one_page = p.page_size % KEYS == 0;   // a step's keys lie in one page
+    const int lrow = lane / CH, lcol = (lane % CH) * 8;
+
+    // The page of my key of the step at (lb, lt); looked up one step ahead, so that its latency is not waited for.
+    // `found`: the key is visible and its page known; `lrow_in`: its row there.
+    int page = 0, row_in = 0;
+    bool found = false;
+    auto look_up = [&]() {
+        const int key = lt * C::kTile + warp * KEYS + (lane % KEYS);
+        found = key >= lr.lo && key < lr.hi;
+        if (found) {
+            const int at = static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(key)) * p.page_mul) >> p.page_shift);
+            page = p.table[lb * p.table_stride + at];
+            row_in = key - at * p.page_size;
+        }
+    };
+    look_up();
 
     auto load_step = [&](int stage) {
         if (to_load > 0) {
-            const int key0 = lt * C::kTile + warp * KEYS;
-            // each lane looks up the page of one key
-            const int key = key0 + (lane % KEYS);
-            bool ok = key >= lr.lo && key < lr.hi;
-            long long ko = 0, vo = 0;
-            if (ok) {
-                const int at = key / p.page_size;
-                const int page = p.table[lb * p.table_stride + at], row = key - at * p.page_size;
-                ok = page >= 0 && page < p.num_pages;
-                if (ok) {
-                    ko = page * p.k_page + row * p.k_row;
-                    vo = page * p.v_page + row * p.v_row;
-                }
-            }
-            const uint32_t mask = __ballot_sync(0xffffffffu, ok);
-            const int hk = lu / p.row_blocks;
-            const uint16_t* kb = p.k + hk * p.k_head;
-            const uint16_t* vb = p.v + hk * p.v_head;
+            const uint32_t mask = __ballot_sync(0xffffffffu, found && page >= 0 && page < p.num_pages);
+            const int hk = p.row_blocks == 1 ? lu : lu / p.row_blocks;
+            const uint16_t* kb = p.k + hk * p.k_head + lcol;
+            const uint16_t* vb = p.v + hk * p.v_head + lcol;
             const uint32_t dst = ring_u + stage * C::kStageBytes;
-            constexpr int CH = D / 8;                        // 16-byte chunks of a row
-            constexpr int RPI = 32 / CH;                     // rows of one instruction
+            if (one_page) {
+                // the first key that can be seen names the page; rows ahead of it and behind the last are not read
+                const int from = mask != 0 ? __ffs(mask) - 1 : 0;
+                const long long pg = mask != 0 ? __shfl_sync(0xffffffffu, page, from) : 0;
+                const int r0 = __shfl_sync(0xffffffffu, row_in, from) - from + lrow;
+                kb += pg * p.k_page + r0 * p.k_row;
+                vb += pg * p.v_page + r0 * p.v_row;
 #pragma unroll
-            for (int i = 0; i < KEYS / RPI; ++i) {
-                const int row = i * RPI + lane / CH, col = lane % CH;
-                const long long kro = __shfl_sync(0xffffffffu, ko, row), vro = __shfl_sync(0xffffffffu, vo, row);
-                const uint32_t bytes = (mask >> row) & 1u ? 16u : 0u;
-                const uint32_t at = dst + row * (D * 2) + ((col ^ (row & 7)) << 4);
-                cp_async16(at, kb + kro + col * 8, bytes);
-                cp_async16(at + KEYS * D * 2, vb + vro + col * 8, bytes);
+                for (int i = 0; i < KEYS / RPI; ++i) {
+                    const int row = i * RPI + lrow;
+                    const uint32_t bytes = (mask >> row) & 1u ? 16u : 0u;
+                    const uint32_t at = dst + row * (D * 2) + (((lane % CH) ^ (row & 7)) << 4);
+                    cp_async16(at, bytes ? kb : p.k, bytes);
+                    cp_async16(at + KEYS * D * 2, bytes ? vb : p.v, bytes);
+                    kb += RPI * p.k_row;
+                    vb += RPI * p.v_row;
+                }
+            } else {
+                const bool ok = (mask >> (lane % KEYS)) & 1u;
+                const long long ko = ok ? page * p.k_page + row_in * p.k_row : 0, vo = ok ? page * p.v_page + row_in * p.v_row : 0;
+#pragma unroll
+                for (int i = 0; i < KEYS / RPI; ++i) {
+                    const int row = i * RPI + lrow;
+                    const long long kro = __shfl_sync(0xffffffffu, ko, row), vro = __shfl_sync(0xffffffffu, vo, row);
+                    const uint32_t bytes = (mask >> row) & 1u ? 16u : 0u;
+                    const uint32_t at = dst + row * (D * 2) + (((lane % CH) ^ (row & 7)) << 4);
+                    cp_async16(at, kb + kro, bytes);
+                    cp_async16(at + KEYS * D * 2, vb + vro, bytes);
+                }
             }
             if (lane == 0) {
                 Step& st = s_step[warp][stage];
                 st.b = lb;
                 st.unit = lu;
-                st.rel = key0 - (lr.hi - 1);
-                st.mask = mask;
+                st.rel = lt * C::kTile + warp * KEYS - (lr.hi - 1);
+                st.mask = KEYS == 32 ? mask : mask & 0xffffu;
                 st.last = (to_load == 1 ? 1 : 0) | (lt + 1 == lr.tile_hi ? 2 : 0);
             }
-            --to_load;
-            if (++lt == lr.tile_hi) {
-                if (++lu == per_request) {
-                    lu = 0;
-                    if (++lb < p.batch) lr = key_range(p, p.lens[lb], C::kTile);
+            if (--to_load > 0) {
+                if (++lt == lr.tile_hi) {
+                    if (++lu == per_request) {
+                        lu = 0;
+                        ++lb;
+                        lr = key_range<C::kTile>(p, p.lens[lb]);
+                    }
+                    lt = lr.tile_lo;
                 }
-                lt = lr.tile_lo;
+                look_up();
             }
         }
         cp_async_commit();
@@ -720,31 +786,44 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
     for (int s = 0; s < STAGES - 1; ++s) load_step(s);
 
     float o[DT][NT][4], m[NT][2], l[NT][2];
-    uint32_t qf[NT][KK][2];
+    uint32_t qf[C::kQueryInSmem ? 1 : NT][C::kQueryInSmem ? 1 : KK][2];
     float slope[NT][2];
-    const float scale2 = p.scale * kLog2e;
     bool fresh = true;               // a unit begins
     bool from_begin = !first_inside;
     int stage = 0;
-    for (long long left = end - begin; left > 0; --left) {
+    for (int left = static_cast<int>(end - begin); left > 0; --left) {
         __syncwarp();                // every lane has read the stage that is filled next
         load_step(stage == 0 ? STAGES - 1 : stage - 1);
         cp_async_wait<STAGES - 1>();
         __syncwarp();
         const Step st = s_step[warp][stage];
-        const int hk = st.unit / p.row_blocks, row0 = (st.unit % p.row_blocks) * ROWS;   // first query head in the group
+        const int hk = p.row_blocks == 1 ? st.unit : st.unit / p.row_blocks;
+        const int row0 = (st.unit - hk * p.row_blocks) * ROWS;               // first query head in the group
         if (fresh) {
             fresh = false;
+            const uint16_t* qrow = p.q + st.b * p.q_batch + (static_cast<long long>(hk) * p.group + row0) * p.q_head;
+            if constexpr (C::kQueryInSmem) {
+                // all four warps are here: the unit before has been joined, and the first begins with the launch
+                for (int i = tid; i < ROWS * CH; i += kAttnThreads) {
+                    const int r = i / CH, c = i % CH;
+                    const uint4 x = row0 + r < p.group ? ld_v4(qrow + r * p.q_head + c * 8) : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(join) + r * (D * 2) + ((c ^ (r & 7)) << 4)) = x;
+                }
+                __syncthreads();
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int r = n * 8 + lane / 4;
+#pragma unroll
+                    for (int k = 0; k < KK; ++k) {
+                        const uint16_t* x = qrow + r * p.q_head + k * 16 + (lane % 4) * 2;
+                        qf[n][k][0] = row0 + r < p.group ? *reinterpret_cast<const uint32_t*>(x) : 0u;
+                        qf[n][k][1] = row0 + r < p.group ? *reinterpret_cast<const uint32_t*>(x + 8) : 0u;
+                    }
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int r = row0 + n * 8 + lane / 4;
-                const uint16_t* qrow = p.q + st.b * p.q_batch + (static_cast<long long>(hk) * p.group + r) * p.q_head;
-#pragma unroll
-                for (int k = 0; k < KK; ++k) {
-                    const int c = k * 16 + (lane % 4) * 2;
-                    qf[n][k][0] = r < p.group ? *reinterpret_cast<const uint32_t*>(qrow + c) : 0u;
-                    qf[n][k][1] = r < p.group ? *reinterpret_cast<const uint32_t*>(qrow + c + 8) : 0u;
-                }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     m[n][e] = -INFINITY;
@@ -762,18 +841,33 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
         // ---- S^T = K Q^T
         float s[MT][NT][4];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[t][n][e] = 0.f;
-            const int row = t * 16 + (lane & 15);
 #pragma unroll
-            for (int k = 0; k < KK; ++k) {
+        for (int k = 0; k < KK; ++k) {
+            uint32_t qs[NT][2];
+            if constexpr (C::kQueryInSmem) {
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t x[4];
+                    const int r = n * 8 + (lane & 7) + ((lane >> 4) << 3);
+                    ldmatrix_x4(x, join_u + r * (D * 2) + (((k * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+                    qs[n][0] = x[0], qs[n][1] = x[1], qs[n + 1][0] = x[2], qs[n + 1][1] = x[3];
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
                 uint32_t a[4];
+                const int row = t * 16 + (lane & 15);
                 ldmatrix_x4(a, kaddr + row * (D * 2) + (((k * 2 + (lane >> 4)) ^ (row & 7)) << 4));
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma16816<BF16>(s[t][n], a, qf[n][k][0], qf[n][k][1]);
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (C::kQueryInSmem) mma16816<BF16>(s[t][n], a, qs[n][0], qs[n][1]);
+                    else mma16816<BF16>(s[t][n], a, qf[n][k][0], qf[n][k][1]);
+                }
             }
         }
         // ---- scores in powers of two
@@ -789,20 +883,16 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
                 const float back = static_cast<float>(st.rel + key);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float x;
-                    if (p.cap > 0.f) {
-                        // tanh(y) = 1 - 2 / (1 + e^(2y)): exact at both ends, absolute error of 2^-23 around 0
-                        const float y = s[t][n][e] * p.scale / p.cap;
-                        x = p.cap * kLog2e * (1.f - 2.f * rcp_approx(1.f + exp2_approx(2.f * kLog2e * y)));
-                    } else {
-                        x = s[t][n][e] * scale2;
-                    }
+                    float x = s[t][n][e];
+                    if constexpr (CAP) x = fmaf(-2.f * p.cap2, rcp_approx(1.f + exp2_approx(x * p.inner)), p.cap2);
+                    else x *= p.scale2;
                     x = fmaf(slope[n][e & 1], back, x);
                     x = seen ? x : -INFINITY;
                     s[t][n][e] = x;
                     top[n][e & 1] = fmaxf(top[n][e & 1], x);
                 }
             }
+        bool grown = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -811,28 +901,36 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                const float now = fmaxf(m[n][e], x);
-                const float ref = now == -INFINITY ? 0.f : now;
-                const float f = exp2_approx(m[n][e] - ref);
-                m[n][e] = now;
-                top[n][e] = ref;
-                l[n][e] *= f;
-#pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    o[t][n][e] *= f;
-                    o[t][n][e + 2] *= f;
-                }
+                top[n][e] = x;
+                grown |= x > m[n][e];
             }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float now = fmaxf(m[n][e], top[n][e]);
+                    const float f = exp2_approx(m[n][e] - (now == -INFINITY ? 0.f : now));
+                    m[n][e] = now;
+                    l[n][e] *= f;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        o[t][n][e] *= f;
+                        o[t][n][e + 2] *= f;
+                    }
+                }
+        }
         // ---- O^T += V^T P^T
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                const float r0 = m[n][0] == -INFINITY ? 0.f : m[n][0], r1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float p0 = exp2_approx(s[t][n][2 * h] - top[n][0]);
-                    const float p1 = exp2_approx(s[t][n][2 * h + 1] - top[n][1]);
+                    const float p0 = exp2_approx(s[t][n][2 * h] - r0);
+                    const float p1 = exp2_approx(s[t][n][2 * h + 1] - r1);
                     l[n][0] += p0;
                     l[n][1] += p1;
                     const uint32_t w = pack2<BF16>(p0, p1);
@@ -840,16 +938,16 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
                     hi[n][h] = movmatrix(w);
                     lo[n][h] = movmatrix(pack2<BF16>(p0 - back.x, p1 - back.y));
                 }
+            }
             const int row = t * 16 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 uint32_t a[4];
                 ldmatrix_x4_trans(a, vaddr + row * (D * 2) + (((dt * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    mma16816<BF16>(o[dt][n], a, hi[n][0], hi[n][1]);
-                    mma16816<BF16>(o[dt][n], a, lo[n][0], lo[n][1]);
-                }
+                for (int n = 0; n < NT; ++n) mma16816<BF16>(o[dt][n], a, hi[n][0], hi[n][1]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816<BF16>(o[dt][n], a, lo[n][0], lo[n][1]);
             }
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -858,6 +956,7 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
             // ---- the unit ends, or the share does: the four warps' results become one, eight heads at a time
             const bool to_end = (st.last & 2) != 0;
             float* part = p.parts + (2 * static_cast<long long>(share) + (from_begin ? 1 : 0)) * p.part_floats;
+            if constexpr (C::kQueryInSmem) __syncthreads();      // the query rows are not needed any more
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -918,66 +1017,66 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_kernel(const Att
 }
 
 // Joins the parts of the units that several shares worked on.  CTA (x, y): the unit inside which share x + 1
-// begins, if that is the first border inside the unit, row y of it; the warps take the parts in turn.
+// begins, if that is the first border inside the unit, rows y, y + grid.y, ... of it; the warps take the parts in
+// turn.  The maximum over the parts comes first, so that nothing in the loop over the accumulators waits for
+// the part before.
 constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 8;           // rows of a unit that are joined side by side
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnParams p, int rows) {
-    __shared__ float s_o[kJoinThreads / 32][D];
-    __shared__ float s_m[kJoinThreads / 32], s_l[kJoinThreads / 32];
+    constexpr int kJoinWarps = kJoinThreads / 32, V = D / 32;
+    __shared__ float s_o[kJoinWarps][D];
     pdl_launch_dependents();
     pdl_wait_prior_grid();
-    const int share = blockIdx.x + 1, row = blockIdx.y;
+    const int share = blockIdx.x + 1;
     const ShareInfo info = p.info[share];
     if (!info.inside) return;
     const int first = share_of(info.unit_begin, info.total, info.shares);
     if (share != first + 1) return;
-    const int last = share_of(info.unit_end - 1, info.total, info.shares);
+    const int count = share_of(info.unit_end - 1, info.total, info.shares) - first + 1;
     const int per_request = p.heads_k * p.row_blocks;
     const int b = info.unit / per_request, u = info.unit % per_request;
-    const int hk = u / p.row_blocks, head = (u % p.row_blocks) * rows + row;
-    if (head >= p.group) return;
+    const int hk = u / p.row_blocks, row0 = (u % p.row_blocks) * rows;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int V = D / 32;
-    float m = -INFINITY, l = 0.f, o[V];
+    auto part = [&](int i) { return p.parts + (2 * static_cast<long long>(first + i) + (i == 0 ? 1 : 0)) * p.part_floats; };
+    for (int row = blockIdx.y; row < rows && row0 + row < p.group; row += gridDim.y) {
+        float top = -INFINITY;
+        for (int i = lane; i < count; i += 32) top = fmaxf(top, part(i)[rows * D + 2 * row]);
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = 0.f;
-    for (int c = first + warp; c <= last; c += kJoinThreads / 32) {
-        const float* part = p.parts + (2 * static_cast<long long>(c) + (c == first ? 1 : 0)) * p.part_floats;
-        const float pm = part[rows * D + 2 * row], pl = part[rows * D + 2 * row + 1];
-        float x[V];
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        for (int i = lane; i < count; i += 32) {
+            const float* x = part(i) + rows * D + 2 * row;
+            sum = fmaf(exp2_approx(x[0] - ref), x[1], sum);
+        }
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = part[row * D + i * 32 + lane];
-        const float now = fmaxf(m, pm), ref = now == -INFINITY ? 0.f : now;
-        const float f = exp2_approx(m - ref), g = exp2_approx(pm - ref);
-        m = now;
-        l = l * f + pl * g;
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        float acc[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = o[i] * f + x[i] * g;
+        for (int v = 0; v < V; ++v) acc[v] = 0.f;
+#pragma unroll 4
+        for (int i = warp; i < count; i += kJoinWarps) {
+            const float* x = part(i);
+            const float f = exp2_approx(x[rows * D + 2 * row] - ref);
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[v] = fmaf(f, x[row * D + v * 32 + lane], acc[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) s_o[warp][v * 32 + lane] = acc[v];
+        __syncthreads();
+        if (tid < D) {
+            float o = 0.f;
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; ++w) o += s_o[w][tid];
+            const long long h = static_cast<long long>(b) * p.heads + hk * p.group + row0 + row;
+            const float v = sum == 0.f ? 0.f : o / sum;
+            p.out[h * D + tid] = static_cast<uint16_t>(pack2<BF16>(v, 0.f));
+            if (tid == 0 && p.lse != nullptr) p.lse[h] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+        }
+        __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) s_o[warp][i * 32 + lane] = o[i];
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
-    __syncthreads();
-    if (tid >= D) return;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_m[w]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) {
-        const float f = exp2_approx(s_m[w] - ref);
-        sum = fmaf(f, s_l[w], sum);
-        acc = fmaf(f, s_o[w][tid], acc);
-    }
-    const long long h = static_cast<long long>(b) * p.heads + hk * p.group + head;
-    const float v = sum == 0.f ? 0.f : acc / sum;
-    p.out[h * D + tid] = static_cast<uint16_t>(pack2<BF16>(v, 0.f));
-    if (tid == 0 && p.lse != nullptr) p.lse[h] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1088,21 +1187,28 @@ static void fill_rotary(RotaryParams* p, const FaRotarySpec& r) {
 }
 
 template <int D, bool BF16>
-static int launch_rotary(const RotaryParams& p, bool interleaved, long long tokens, int outer, cudaStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(outer));
+static int launch_rotary(RotaryParams p, bool interleaved, long long tokens, int outer, int sms, cudaStream_t stream) {
+    constexpr int kHeadsAtOnce = kRotaryThreads / (D / 16);
+    const long long heads = static_cast<long long>(p.rows[0].heads) + p.rows[1].heads + p.rows[2].heads;
+    p.tokens = static_cast<int>(tokens);
+    p.per_cta = 1;
+    while (p.per_cta < kRotaryTokens && 2 * heads * p.per_cta <= kRotaryBatch * kHeadsAtOnce &&
+           tokens * outer >= 2LL * p.per_cta * kRotaryWaves * sms)
+        p.per_cta *= 2;
+    const dim3 grid(static_cast<unsigned>((tokens + p.per_cta - 1) / p.per_cta), static_cast<unsigned>(outer));
     if (interleaved) return launch_chained(rotary_kernel<D, BF16, kNeighbours>, grid, kRotaryThreads, 0, stream, p);
     if (p.rot % 16 == 0) return launch_chained(rotary_kernel<D, BF16, kHalves>, grid, kRotaryThreads, 0, stream, p);
     return launch_chained(rotary_kernel<D, BF16, kRaggedHalves>, grid, kRotaryThreads, 0, stream, p);
 }
 
 static int launch_rotary(const RotaryParams& p, bool interleaved, long long tokens, int outer, int head_dim, int dtype,
-                         cudaStream_t stream) {
+                         int sms, cudaStream_t stream) {
     const bool bf16 = dtype == FA_PAGED_BF16;
     if (head_dim == 128)
-        return bf16 ? launch_rotary<128, true>(p, interleaved, tokens, outer, stream)
-                    : launch_rotary<128, false>(p, interleaved, tokens, outer, stream);
-    return bf16 ? launch_rotary<64, true>(p, interleaved, tokens, outer, stream)
-                : launch_rotary<64, false>(p, interleaved, tokens, outer, stream);
+        return bf16 ? launch_rotary<128, true>(p, interleaved, tokens, outer, sms, stream)
+                    : launch_rotary<128, false>(p, interleaved, tokens, outer, sms, stream);
+    return bf16 ? launch_rotary<64, true>(p, interleaved, tokens, outer, sms, stream)
+                : launch_rotary<64, false>(p, interleaved, tokens, outer, sms, stream);
 }
 
 struct AttnPlan {
@@ -1133,17 +1239,20 @@ static int check_attention(const FaPagedAttentionArgs* a) {
 }
 
 template <int D>
-static void make_attn_plan(const FaPagedAttentionArgs* a, int sms, AttnPlan* plan) {
+static int make_attn_plan(const FaPagedAttentionArgs* a, int sms, AttnPlan* plan) {
     const int group = a->heads / a->cache.heads_k;
-    plan->nt = group <= 8 ? 1 : 2;
+    plan->nt = group <= 8 ? 1 : group <= 16 ? 2 : 4;
     plan->row_blocks = (group + plan->nt * 8 - 1) / (plan->nt * 8);
-    const long long tiles = (static_cast<long long>(a->table_width) * a->cache.page_size + AttnCfg<D>::kTile - 1) / AttnCfg<D>::kTile;
+    const long long tiles = (static_cast<long long>(a->table_width) * a->cache.page_size + attn_tile(D) - 1) / attn_tile(D);
     const long long most = static_cast<long long>(a->batch) * a->cache.heads_k * plan->row_blocks * (tiles > 0 ? tiles : 1);
-    const long long resident = 2LL * sms;
+    const long long resident = static_cast<long long>(D == 64 && plan->nt == 1 ? AttnCfg<64, 1>::kCtas : AttnCfg<D, 2>::kCtas) * sms;
+    // tiles of one request, and of one share, are counted in 32 bits
+    if (tiles * a->cache.heads_k * plan->row_blocks > INT_MAX || most / resident >= INT_MAX) return FA_PAGED_ERR_SHAPE;
     plan->grid = static_cast<int>(most < resident ? most : resident);
     plan->part_floats = plan->nt * 8 * (D + 2);
     plan->info_bytes = (plan->grid * sizeof(ShareInfo) + 255) / 256 * 256;
     plan->bytes = plan->info_bytes + 2 * plan->grid * plan->part_floats * sizeof(float);
+    return FA_PAGED_OK;
 }
 
 static int attn_plan(const FaPagedAttentionArgs* a, AttnPlan* plan) {
@@ -1153,26 +1262,34 @@ static int attn_plan(const FaPagedAttentionArgs* a, AttnPlan* plan) {
     if (a->batch == 0 || a->heads == 0) return FA_PAGED_OK;
     const int sms = sm_count(a->device);
     if (sms < 0) return sms;
-    if (a->cache.head_dim == 128) make_attn_plan<128>(a, sms, plan);
-    else make_attn_plan<64>(a, sms, plan);
-    return FA_PAGED_OK;
+    return a->cache.head_dim == 128 ? make_attn_plan<128>(a, sms, plan) : make_attn_plan<64>(a, sms, plan);
 }
 
-template <int D, bool BF16, int NT>
+template <int D, bool BF16, int NT, bool CAP>
 static int launch_attention(const AttnParams& p, const AttnPlan& plan, int device, cudaStream_t stream) {
     static std::atomic<unsigned long long> done{0};
-    int rc = allow_smem(paged_attention_kernel<D, BF16, NT>, AttnCfg<D>::kSmem, done, device);
+    constexpr int smem = AttnCfg<D, NT>::kSmem;
+    int rc = allow_smem(paged_attention_kernel<D, BF16, NT, CAP>, smem, done, device);
     if (rc != FA_PAGED_OK) return rc;
-    rc = launch_chained(paged_attention_kernel<D, BF16, NT>, dim3(plan.grid), kAttnThreads, AttnCfg<D>::kSmem, stream, p);
+    rc = launch_chained(paged_attention_kernel<D, BF16, NT, CAP>, dim3(plan.grid), kAttnThreads, smem, stream, p);
     if (rc != FA_PAGED_OK || plan.grid < 2) return rc;
-    const int rows = p.group < NT * 8 ? p.group : NT * 8;
+    const int rows = p.group < kJoinRows ? p.group : kJoinRows;
     return launch_chained(paged_join_kernel<D, BF16>, dim3(plan.grid - 1, rows), kJoinThreads, 0, stream, p, NT * 8);
 }
 
+template <int D, bool BF16, int NT>
+static int launch_attention(const AttnParams& p, const AttnPlan& plan, bool cap, int device, cudaStream_t stream) {
+    return cap ? launch_attention<D, BF16, NT, true>(p, plan, device, stream)
+               : launch_attention<D, BF16, NT, false>(p, plan, device, stream);
+}
+
 template <int D, bool BF16>
-static int dispatch_attention(const AttnParams& p, const AttnPlan& plan, int device, cudaStream_t stream) {
-    return plan.nt == 1 ? launch_attention<D, BF16, 1>(p, plan, device, stream)
-                        : launch_attention<D, BF16, 2>(p, plan, device, stream);
+static int dispatch_attention(const AttnParams& p, const AttnPlan& plan, bool cap, int device, cudaStream_t stream) {
+    switch (plan.nt) {
+        case 1: return launch_attention<D, BF16, 1>(p, plan, cap, device, stream);
+        case 2: return launch_attention<D, BF16, 2>(p, plan, cap, device, stream);
+        default: return launch_attention<D, BF16, 4>(p, plan, cap, device, stream);
+    }
 }
 
 static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t bytes, cudaStream_t stream) {
@@ -1199,16 +1316,24 @@ static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t byte
     p.v_page = c.v_page_stride, p.v_head = c.v_head_stride, p.v_row = c.v_row_stride;
     p.batch = a->batch, p.heads = a->heads, p.heads_k = c.heads_k, p.group = a->heads / c.heads_k;
     p.row_blocks = plan.row_blocks, p.width = a->table_width, p.page_size = c.page_size, p.num_pages = c.num_pages;
-    p.window = a->window, p.scale = a->scale, p.cap = a->softcap;
+    p.window = a->window;
+    const bool cap = a->softcap > 0.f;
+    p.scale2 = a->scale * kLog2e;
+    p.cap2 = a->softcap * kLog2e;
+    p.inner = cap ? static_cast<float>(2.0 * 1.4426950408889634 * a->scale / a->softcap) : 0.f;
+    int s = 0;
+    while ((1LL << s) < c.page_size) ++s;
+    p.page_mul = static_cast<unsigned>(((1ULL << (31 + s)) + c.page_size - 1) / c.page_size);
+    p.page_shift = 31 + s;
     p.info = static_cast<ShareInfo*>(workspace);
     p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.info_bytes);
     p.part_floats = plan.part_floats;
     const bool bf16 = a->dtype == FA_PAGED_BF16;
     if (c.head_dim == 128)
-        return bf16 ? dispatch_attention<128, true>(p, plan, a->device, stream)
-                    : dispatch_attention<128, false>(p, plan, a->device, stream);
-    return bf16 ? dispatch_attention<64, true>(p, plan, a->device, stream)
-                : dispatch_attention<64, false>(p, plan, a->device, stream);
+        return bf16 ? dispatch_attention<128, true>(p, plan, cap, a->device, stream)
+                    : dispatch_attention<128, false>(p, plan, cap, a->device, stream);
+    return bf16 ? dispatch_attention<64, true>(p, plan, cap, a->device, stream)
+                : dispatch_attention<64, false>(p, plan, cap, a->device, stream);
 }
 
 static int rotary(const FaRotaryArgs* a, cudaStream_t stream) {
@@ -1244,7 +1369,7 @@ static int rotary(const FaRotaryArgs* a, cudaStream_t stream) {
     p.rows[1] = Rows{static_cast<const uint16_t*>(a->k), static_cast<uint16_t*>(a->k_out), a->k_batch_stride,
                      a->k_head_stride, a->k_row_stride, a->heads_k * plane, plane, d, a->heads_k};
     p.position_outer = a->position_batch_stride;
-    return launch_rotary(p, a->rotary.interleaved != 0, a->seqlen, a->batch, a->head_dim, a->dtype, stream);
+    return launch_rotary(p, a->rotary.interleaved != 0, a->seqlen, a->batch, a->head_dim, a->dtype, sms, stream);
 }
 
 static int append(const FaPagedAppendArgs* a, cudaStream_t stream) {
@@ -1288,7 +1413,7 @@ static int append(const FaPagedAppendArgs* a, cudaStream_t stream) {
     p.slots_64 = a->slots_64 != 0;
     p.page_size = c.page_size;
     p.num_slots = static_cast<long long>(c.num_pages) * c.page_size;
-    return launch_rotary(p, turned && a->rotary.interleaved != 0, a->num_tokens, 1, c.head_dim, a->dtype, stream);
+    return launch_rotary(p, turned && a->rotary.interleaved != 0, a->num_tokens, 1, c.head_dim, a->dtype, sms, stream);
 }
 
 template <typename Args>

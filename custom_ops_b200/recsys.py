@@ -436,6 +436,7 @@ class RecsysOps:
         self._allow_jit = bool(allow_jit)
         self._groups: dict = {}          # name -> CustomOps instance, once somebody asked for it
         self._lock = threading.RLock()
+        self._paged_ops: dict = {}       # name -> operator of the loaded "paged" group
 
     # ---- policy
     @property
@@ -594,6 +595,14 @@ class RecsysOps:
         return self._dispatch(backend, "fa").mha_fwd_rule_mask(q, k, v, bool(causal), int(window), valid_lens)
 
     # ---- the paged key/value cache (no counterpart in the reference)
+    def _paged_call(self, backend, name: str):
+        """``_dispatch`` for calls of a few microseconds: the operator is looked up once."""
+        _resolve_backend(backend)
+        op = self._paged_ops.get(name)
+        if op is None:
+            op = self._paged_ops[name] = getattr(self._dispatch(backend, "paged"), name).default
+        return op
+
     def paged_extend(self, block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,
                      free_pages: torch.Tensor, free_head: torch.Tensor, page_size: int, num_tokens: int,
                      backend: Optional[str] = None):
@@ -609,7 +618,7 @@ class RecsysOps:
         and head, and for the ``num_tokens`` packed new tokens their slot (int64, ``page * page_size + row``;
         -1 for a refused request and behind the last token), their position, and where each request's begin
         (``cu``, ``(B + 1,)``).  Only ``block_table`` is written in place: the call may be repeated."""
-        return self._dispatch(backend, "paged").paged_extend(block_table, seq_lens, new_lens, free_pages, free_head,
+        return self._paged_call(backend, "paged_extend")(block_table, seq_lens, new_lens, free_pages, free_head,
                                                              page_size, num_tokens)
 
     def paged_extend_(self, block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,
@@ -617,7 +626,7 @@ class RecsysOps:
                       backend: Optional[str] = None):
         """``paged_extend`` that updates ``seq_lens`` and ``free_head`` in place - what a captured decoding
         loop wants - and returns ``(slots, positions, cu)``."""
-        return self._dispatch(backend, "paged").paged_extend_(block_table, seq_lens, new_lens, free_pages, free_head,
+        return self._paged_call(backend, "paged_extend_")(block_table, seq_lens, new_lens, free_pages, free_head,
                                                               page_size, num_tokens)
 
     def paged_shrink_(self, block_table: torch.Tensor, seq_lens: torch.Tensor, keep_lens: torch.Tensor,
@@ -625,7 +634,7 @@ class RecsysOps:
                       backend: Optional[str] = None) -> None:
         """Shortens every request to at most ``keep_lens`` tokens (0 releases it) and puts the pages behind that
         back in front of ``free_head``.  ``seq_lens``, ``free_pages`` and ``free_head`` change in place."""
-        return self._dispatch(backend, "paged").paged_shrink_(block_table, seq_lens, keep_lens, free_pages, free_head,
+        return self._paged_call(backend, "paged_shrink_")(block_table, seq_lens, keep_lens, free_pages, free_head,
                                                               page_size)
 
     def rotary(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,
@@ -637,7 +646,7 @@ class RecsysOps:
         (``paged.rotary_frequencies``): ``2 * len(freqs)`` elements of each head turn, in pairs ``(i, i + n)``
         or, ``interleaved``, ``(2i, 2i + 1)``; the rest pass through.  Pairs are scaled by ``mscale``.  Nothing
         here records gradients; ``adjoint`` turns the other way, which is the gradient with respect to q and k."""
-        return self._dispatch(backend, "paged").rotary(q, k, positions, freqs, interleaved, mscale, adjoint)
+        return self._paged_call(backend, "rotary")(q, k, positions, freqs, interleaved, mscale, adjoint)
 
     def rotary_append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
                       slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, freqs: torch.Tensor,
@@ -645,13 +654,13 @@ class RecsysOps:
         """Rotary positions on packed new tokens - q ``(T, H, d)``, k, v ``(T, Hk, d)``, strided views welcome -
         and their keys and values written to ``slots`` of the caches ``(pages, Hk, page_size, d)``.  Returns the
         turned q; a token whose slot is negative or behind the cache is not written."""
-        return self._dispatch(backend, "paged").rotary_append(q, k, v, positions, slots, k_cache, v_cache, freqs,
+        return self._paged_call(backend, "rotary_append")(q, k, v, positions, slots, k_cache, v_cache, freqs,
                                                               interleaved, mscale)
 
     def paged_append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
                      v_cache: torch.Tensor, backend: Optional[str] = None) -> None:
         """``rotary_append`` without the rotation, for models that have none."""
-        return self._dispatch(backend, "paged").paged_append(k, v, slots, k_cache, v_cache)
+        return self._paged_call(backend, "paged_append")(k, v, slots, k_cache, v_cache)
 
     def paged_attention(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                         block_table: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
@@ -665,7 +674,7 @@ class RecsysOps:
         score x into ``softcap * tanh(x / softcap)``; ``slopes`` (fp32, one per head) add
         ``slope * (key - newest key)``; ``window > 0`` hides all but the last ``window`` keys.
         A request without a key gives 0."""
-        return self._dispatch(backend, "paged").paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale,
+        return self._paged_call(backend, "paged_attention")(q, k_cache, v_cache, block_table, seq_lens, scale,
                                                                 window, softcap, slopes)
 
     def paged_attention_lse(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -674,5 +683,5 @@ class RecsysOps:
                             backend: Optional[str] = None):
         """``paged_attention`` that also returns each head's natural log-sum-exp, fp32 ``(B, H)``, ``-inf`` for a
         request without a key: what a join with another part of the keys needs."""
-        return self._dispatch(backend, "paged").paged_attention_lse(q, k_cache, v_cache, block_table, seq_lens, scale,
+        return self._paged_call(backend, "paged_attention_lse")(q, k_cache, v_cache, block_table, seq_lens, scale,
                                                                     window, softcap, slopes)

@@ -28,7 +28,9 @@ namespace fa_paged {
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-// Lets the next kernel of the stream become resident / waits until the kernel before has finished.
+// Lets the next kernel of the stream become resident / waits until the kernel before has finished.  The attention
+// kernels do not announce the next one early: resident CTAs of the next take their places SM by SM as theirs
+// leave, which spread the next call unevenly (48 requests, 16 heads of 64: 53 us a call with it, 40 without).
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -519,9 +521,10 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
 // ------------------------------------------------------------------------------------------------
 // Attention of one new token per request over the pages
 // ------------------------------------------------------------------------------------------------
-// Mathematics: one pass over the keys with a running maximum m, sum l and accumulator o per query head, in
-// fp32 and in powers of two: x = log2(e) * score, p = 2^(x - m), o = sum p v.  Parts of a key range are joined
-// by  o = sum_i 2^(m_i - m) o_i  and likewise l.
+// Mathematics: one pass over the keys with a running reference m, a sum l and an accumulator o per query head, in
+// fp32 and in powers of two: x = log2(e) * score, p = 2^(x - m), l = sum p, o = sum p v.  m is a maximum that moves
+// only when a score exceeds it by more than 8 (p stays below 2^8, and o / l does not depend on m).  Parts of a
+// key range are joined by  o = sum_i 2^(m_i - m) o_i  and likewise l.
 //
 // Bound: memory.  A key of a KV head costs 4 * head_dim bytes and 4 * head_dim flops per query head of the
 // group, so even 32 heads a group stay far from the tensor pipe's balance (250 flops a byte).  What matters is
@@ -550,6 +553,7 @@ constexpr int kWarps = 4;
 constexpr int kAttnThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kGrowth = 8.f;         // how far (in powers of two) a score may exceed the reference m
 
 template <int D, int NT>
 struct AttnCfg {
@@ -581,6 +585,7 @@ struct AttnParams {
     long long q_batch, q_head, table_stride;
     long long k_page, k_head, k_row, v_page, v_head, v_row;
     int batch, heads, heads_k, group, row_blocks, width, page_size, num_pages, window;
+    int whole;                    // 1: CTA u does unit u from its first key to its last
     unsigned page_mul, page_shift;      // key / page_size = key * page_mul >> page_shift, for keys below 2^31
     // x, in powers of two, is s * scale2, or with a cap  cap2 * tanh(s * inner / 2),  inner = 2 log2(e) scale / cap:
     // tanh(y) = 1 - 2 / (1 + 2^(2 log2(e) y))
@@ -624,69 +629,81 @@ __device__ __forceinline__ int share_of(long long at, long long total, int share
     return static_cast<int>(((at + 1) * shares - 1) / total);
 }
 
+template <bool BF16>
+__device__ __forceinline__ uint2 pack4(float4 x) { return make_uint2(pack2<BF16>(x.x, x.y), pack2<BF16>(x.z, x.w)); }
+__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ void store_lse(const AttnParams& p, long long head, float sum, float top) {
+    if (p.lse != nullptr) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
 template <int D, bool BF16, int NT, bool CAP>
 __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_attention_kernel(const AttnParams p) {
     using C = AttnCfg<D, NT>;
     constexpr int MT = C::kKeys / 16, KK = D / 16, DT = D / 16, KEYS = C::kKeys, STAGES = C::kStages;
     constexpr int ROWS = NT * 8;
     extern __shared__ __align__(128) uint8_t s_ring[];
-    __shared__ long long s_scan[kWarps];
-    __shared__ long long s_start[2];
-    __shared__ float s_m[kWarps][8], s_l[kWarps][8];
-    struct Step { int b, unit, rel, last; uint32_t mask; int pad[3]; };
+    __shared__ long long s_scan[kWarps], s_at, s_total;
+    __shared__ int s_request, s_len;
+    __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+    struct Step { int b, unit, rel, last; uint32_t mask; int pad[3]; };     // last: 1 ends the share, 2 ends its unit
     __shared__ Step s_step[kWarps][STAGES];
-    pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per_request = p.heads_k * p.row_blocks;
+    const int per_request = p.heads_k * p.row_blocks, share = blockIdx.x;
 
-    // ---- my share
-    const int chunk = (p.batch + kAttnThreads - 1) / kAttnThreads;
-    const int b_lo = min(tid * chunk, p.batch), b_hi = min(b_lo + chunk, p.batch);
-    long long mine = 0;
-    for (int b = b_lo; b < b_hi; ++b) {
-        const Range r = key_range<C::kTile>(p, p.lens[b]);
-        mine += static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
-    }
-    const long long upto = block_scan(mine, s_scan);
-    if (tid == kAttnThreads - 1) s_start[0] = upto;
-    __syncthreads();
-    const long long total = s_start[0];
-    const int shares = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-    const int share = blockIdx.x;
-    if (share >= shares) {
-        if (tid == 0) p.info[share].inside = 0;
-        return;
-    }
-    const long long begin = share_begin(share, total, shares), end = share_begin(share + 1, total, shares);
-    __syncthreads();
-    if (begin >= upto - mine && begin < upto) {
-        long long at = upto - mine;
+    // ---- my share; the loader's place: request, unit within the request, tile
+    int lb, lu, lt, to_load;
+    Range lr;
+    if (p.whole) {
+        lb = share / per_request;
+        lu = share - lb * per_request;
+        lr = key_range<C::kTile>(p, p.lens[lb]);
+        lt = lr.tile_lo;
+        to_load = lr.tile_hi - lt;
+    } else {
+        const int chunk = (p.batch + kAttnThreads - 1) / kAttnThreads;
+        const int b_lo = min(tid * chunk, p.batch), b_hi = min(b_lo + chunk, p.batch);
+        long long mine = 0;
         for (int b = b_lo; b < b_hi; ++b) {
             const Range r = key_range<C::kTile>(p, p.lens[b]);
-            const long long n = static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
-            if (begin < at + n) {
-                s_start[0] = b;
-                s_start[1] = at;
-                break;
-            }
-            at += n;
+            mine += static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
         }
-    }
-    __syncthreads();
-
-    // ---- the loader's place: request, unit within the request, tile
-    int lb = static_cast<int>(s_start[0]);
-    Range lr = key_range<C::kTile>(p, p.lens[lb]);
-    int lu, lt;
-    {
-        const unsigned off = static_cast<unsigned>(begin - s_start[1]);     // below tiles * per_request: 31 bits, checked
+        const long long upto = block_scan(mine, s_scan);
+        if (tid == kAttnThreads - 1) s_total = upto;
+        __syncthreads();
+        const long long total = s_total;
+        const int shares = total < gridDim.x ? static_cast<int>(total) : static_cast<int>(gridDim.x);
+        if (share >= shares) {
+            if (tid == 0) p.info[share].inside = 0;
+            return;
+        }
+        const long long begin = share_begin(share, total, shares);
+        to_load = static_cast<int>(share_begin(share + 1, total, shares) - begin);
+        if (begin >= upto - mine && begin < upto) {
+            long long at = upto - mine;
+            for (int b = b_lo; b < b_hi; ++b) {
+                const int len = p.lens[b];
+                const Range r = key_range<C::kTile>(p, len);
+                const long long n = static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
+                if (begin < at + n) {
+                    s_request = b;
+                    s_len = len;
+                    s_at = at;
+                    break;
+                }
+                at += n;
+            }
+        }
+        __syncthreads();
+        lb = s_request;
+        lr = key_range<C::kTile>(p, s_len);
+        const unsigned off = static_cast<unsigned>(begin - s_at);     // below tiles * per_request: 31 bits, checked
         const unsigned tiles = lr.tile_hi - lr.tile_lo;
         lu = off / tiles;
-        lt = lr.tile_lo + off % tiles;
+        lt = lr.tile_lo + off - lu * tiles;
         if (tid == 0) {
             ShareInfo info;
-            info.unit_begin = s_start[1] + static_cast<long long>(lu) * tiles;
+            info.unit_begin = s_at + static_cast<long long>(lu) * tiles;
             info.unit_end = info.unit_begin + tiles;
             info.total = total;
             info.unit = lb * per_request + lu;
@@ -696,8 +713,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
             p.info[share] = info;
         }
     }
-    const bool first_inside = lt > lr.tile_lo;       // the share begins inside a unit
-    int to_load = static_cast<int>(end - begin);
+    bool from_begin = lt == lr.tile_lo;              // this part of a unit contains its first key
 
     const uint32_t ring_u = smem_u32(s_ring) + warp * (C::kStageBytes * STAGES);
     float* join = reinterpret_cast<float*>(s_ring + C::kRingBytes);
@@ -709,7 +725,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     const int lrow = lane / CH, lcol = (lane % CH) * 8;
 
     // The page of my key of the step at (lb, lt); looked up one step ahead, so that its latency is not waited for.
-    // `found`: the key is visible and its page known; `lrow_in`: its row there.
+    // `found`: the key is visible; `row_in`: its row in the page.
     int page = 0, row_in = 0;
     bool found = false;
     auto look_up = [&]() {
@@ -723,13 +739,20 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     };
     look_up();
 
-    auto load_step = [&](int stage) {
+    float o[DT][NT][4], m[NT][2], l[NT][2];
+    uint32_t qf[C::kQueryInSmem ? 1 : NT][C::kQueryInSmem ? 1 : KK][2];
+    bool fresh = true;               // a unit begins
+    int stage = 0, ahead = STAGES - 1;               // steps to load before the first is waited for
+    for (;;) {
+        // ---- load the step that is STAGES - 1 ahead
+        __syncwarp();                // every lane has read the stage that is filled
         if (to_load > 0) {
             const uint32_t mask = __ballot_sync(0xffffffffu, found && page >= 0 && page < p.num_pages);
             const int hk = p.row_blocks == 1 ? lu : lu / p.row_blocks;
             const uint16_t* kb = p.k + hk * p.k_head + lcol;
             const uint16_t* vb = p.v + hk * p.v_head + lcol;
-            const uint32_t dst = ring_u + stage * C::kStageBytes;
+            const int load_stage = ahead > 0 ? STAGES - 1 - ahead : stage == 0 ? STAGES - 1 : stage - 1;
+            const uint32_t dst = ring_u + load_stage * C::kStageBytes;
             if (one_page) {
                 // the first key that can be seen names the page; rows ahead of it and behind the last are not read
                 const int from = mask != 0 ? __ffs(mask) - 1 : 0;
@@ -750,7 +773,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
             } else {
                 const bool ok = (mask >> (lane % KEYS)) & 1u;
                 const long long ko = ok ? page * p.k_page + row_in * p.k_row : 0, vo = ok ? page * p.v_page + row_in * p.v_row : 0;
-#pragma unroll
+#pragma unroll 2
                 for (int i = 0; i < KEYS / RPI; ++i) {
                     const int row = i * RPI + lrow;
                     const long long kro = __shfl_sync(0xffffffffu, ko, row), vro = __shfl_sync(0xffffffffu, vo, row);
@@ -761,7 +784,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
                 }
             }
             if (lane == 0) {
-                Step& st = s_step[warp][stage];
+                Step& st = s_step[warp][load_stage];
                 st.b = lb;
                 st.unit = lu;
                 st.rel = lt * C::kTile + warp * KEYS - (lr.hi - 1);
@@ -781,20 +804,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
             }
         }
         cp_async_commit();
-    };
-
-    for (int s = 0; s < STAGES - 1; ++s) load_step(s);
-
-    float o[DT][NT][4], m[NT][2], l[NT][2];
-    uint32_t qf[C::kQueryInSmem ? 1 : NT][C::kQueryInSmem ? 1 : KK][2];
-    float slope[NT][2];
-    bool fresh = true;               // a unit begins
-    bool from_begin = !first_inside;
-    int stage = 0;
-    for (int left = static_cast<int>(end - begin); left > 0; --left) {
-        __syncwarp();                // every lane has read the stage that is filled next
-        load_step(stage == 0 ? STAGES - 1 : stage - 1);
-        cp_async_wait<STAGES - 1>();
+        if (ahead > 0) {
+            --ahead;
+            continue;
+        }
         __syncwarp();
         const Step st = s_step[warp][stage];
         const int hk = p.row_blocks == 1 ? st.unit : st.unit / p.row_blocks;
@@ -828,8 +841,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
                 for (int e = 0; e < 2; ++e) {
                     m[n][e] = -INFINITY;
                     l[n][e] = 0.f;
-                    const int rr = row0 + n * 8 + (lane % 4) * 2 + e;
-                    slope[n][e] = p.slopes != nullptr && rr < p.group ? p.slopes[hk * p.group + rr] * kLog2e : 0.f;
                 }
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
@@ -837,6 +848,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
                     for (int e = 0; e < 4; ++e) o[t][n][e] = 0.f;
             }
         }
+        cp_async_wait<STAGES - 1>();
+        __syncwarp();
         const uint32_t kaddr = ring_u + stage * C::kStageBytes, vaddr = kaddr + KEYS * D * 2;
         // ---- S^T = K Q^T
         float s[MT][NT][4];
@@ -871,52 +884,68 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
             }
         }
         // ---- scores in powers of two
-        float top[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int key = t * 16 + lane / 4 + (e >> 1) * 8;
-                const bool seen = (st.mask >> key) & 1u;
-                const float back = static_cast<float>(st.rel + key);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float x = s[t][n][e];
-                    if constexpr (CAP) x = fmaf(-2.f * p.cap2, rcp_approx(1.f + exp2_approx(x * p.inner)), p.cap2);
-                    else x *= p.scale2;
-                    x = fmaf(slope[n][e & 1], back, x);
-                    x = seen ? x : -INFINITY;
-                    s[t][n][e] = x;
-                    top[n][e & 1] = fmaxf(top[n][e & 1], x);
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (CAP) s[t][n][e] = fmaf(-2.f * p.cap2, rcp_approx(1.f + exp2_approx(s[t][n][e] * p.inner)), p.cap2);
+                    else s[t][n][e] *= p.scale2;
                 }
-            }
+        if (p.slopes != nullptr) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = row0 + n * 8 + (lane % 4) * 2 + r;
+                    const float slope = row < p.group ? p.slopes[hk * p.group + row] * kLog2e : 0.f;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                        for (int e = r; e < 4; e += 2)
+                            s[t][n][e] = fmaf(slope, static_cast<float>(st.rel + t * 16 + lane / 4 + (e >> 1) * 8), s[t][n][e]);
+                }
+        }
+        if (st.mask != (KEYS == 32 ? 0xffffffffu : 0xffffu)) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool seen = (st.mask >> (t * 16 + lane / 4 + (e >> 1) * 8)) & 1u;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) s[t][n][e] = seen ? s[t][n][e] : -INFINITY;
+                }
+        }
+        float top[NT][2];
         bool grown = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float x = top[n][e];
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                top[n][e] = x;
-                grown |= x > m[n][e];
+            for (int r = 0; r < 2; ++r) {
+                float x = fmaxf(s[0][n][r], s[0][n][r + 2]);
+#pragma unroll
+                for (int t = 1; t < MT; ++t) x = fmaxf(x, fmaxf(s[t][n][r], s[t][n][r + 2]));
+                top[n][r] = x;
+                grown |= x > m[n][r] + kGrowth;
             }
         if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float now = fmaxf(m[n][e], top[n][e]);
-                    const float f = exp2_approx(m[n][e] - (now == -INFINITY ? 0.f : now));
-                    m[n][e] = now;
-                    l[n][e] *= f;
+                for (int r = 0; r < 2; ++r) {
+                    float x = top[n][r];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float now = fmaxf(m[n][r], x);
+                    const float f = exp2_approx(m[n][r] - finite_ref(now));
+                    m[n][r] = now;
+                    l[n][r] *= f;
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
-                        o[t][n][e] *= f;
-                        o[t][n][e + 2] *= f;
+                        o[t][n][r] *= f;
+                        o[t][n][r + 2] *= f;
                     }
                 }
         }
@@ -926,7 +955,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
             uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float r0 = m[n][0] == -INFINITY ? 0.f : m[n][0], r1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+                const float r0 = finite_ref(m[n][0]), r1 = finite_ref(m[n][1]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float p0 = exp2_approx(s[t][n][2 * h] - r0);
@@ -951,131 +980,177 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
             }
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
+        if (st.last == 0) continue;
 
-        if (st.last != 0) {
-            // ---- the unit ends, or the share does: the four warps' results become one, eight heads at a time
-            const bool to_end = (st.last & 2) != 0;
-            float* part = p.parts + (2 * static_cast<long long>(share) + (from_begin ? 1 : 0)) * p.part_floats;
-            if constexpr (C::kQueryInSmem) __syncthreads();      // the query rows are not needed any more
+        // ---- the unit ends, or the share does: the four warps' results become one.  Each warp scales its own to the
+        // maximum of the four; what is left is a sum, eight heads at a time through shared memory.
+        const bool whole = from_begin && (st.last & 2) != 0;
+        const int rows = min(p.group - row0, ROWS);
+        const long long head0 = static_cast<long long>(st.b) * p.heads + hk * p.group + row0;
+        float* const part = p.parts + (2 * static_cast<long long>(share) + (from_begin ? 1 : 0)) * p.part_floats;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float x = l[n][e];
-                    x += __shfl_xor_sync(0xffffffffu, x, 4);
-                    x += __shfl_xor_sync(0xffffffffu, x, 8);
-                    x += __shfl_xor_sync(0xffffffffu, x, 16);
-                    const int r = (lane % 4) * 2 + e;
-                    if (lane < 4) {
-                        s_m[warp][r] = m[n][e];
-                        s_l[warp][r] = x;
-                    }
+            for (int r = 0; r < 2; ++r) {
+                float x = l[n][r];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (lane < 4) {
+                    s_m[warp][n * 8 + lane * 2 + r] = m[n][r];
+                    s_l[warp][n * 8 + lane * 2 + r] = x;
+                }
+            }
+        __syncthreads();             // (and, with the query rows in shared memory: they are not needed any more)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (n * 8 >= rows) break;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = n * 8 + (lane % 4) * 2 + r;
+                const float most = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+                const float f = exp2_approx(m[n][r] - finite_ref(most));
+                if (row < rows)
 #pragma unroll
                     for (int t = 0; t < DT; ++t)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int d = t * 16 + h * 8 + lane / 4;
-                            join[(warp * 8 + r) * D + (d ^ ((lane % 4) * 8))] = o[t][n][e + 2 * h];
-                        }
-                }
-                __syncthreads();
-                for (int i = tid; i < 8 * D; i += kAttnThreads) {
-                    const int r = i / D, d = i % D, head = row0 + n * 8 + r;
-                    if (head >= p.group) break;
-                    float top4 = s_m[0][r];
-#pragma unroll
-                    for (int w = 1; w < kWarps; ++w) top4 = fmaxf(top4, s_m[w][r]);
-                    const float ref = top4 == -INFINITY ? 0.f : top4;
-                    float sum = 0.f, acc = 0.f;
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) {
-                        const float f = exp2_approx(s_m[w][r] - ref);
-                        sum = fmaf(f, s_l[w][r], sum);
-                        acc = fmaf(f, join[(w * 8 + r) * D + (d ^ ((r >> 1) * 8))], acc);
-                    }
-                    if (from_begin && to_end) {
-                        const long long h = static_cast<long long>(st.b) * p.heads + hk * p.group + head;
-                        const float v = sum == 0.f ? 0.f : acc / sum;
-                        p.out[h * D + d] = static_cast<uint16_t>(pack2<BF16>(v, 0.f));
-                        if (d == 0 && p.lse != nullptr)
-                            p.lse[h] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
-                    } else {
-                        part[(n * 8 + r) * D + d] = acc;
-                        if (d == 0) {
-                            part[ROWS * D + 2 * (n * 8 + r)] = top4;
-                            part[ROWS * D + 2 * (n * 8 + r) + 1] = sum;
-                        }
-                    }
-                }
-                __syncthreads();
+                        for (int h = 0; h < 2; ++h)
+                            join[(warp * 8 + (lane % 4) * 2 + r) * D + ((t * 16 + h * 8 + lane / 4) ^ ((lane % 4) * 8))] = o[t][n][r + 2 * h] * f;
             }
-            fresh = true;
-            from_begin = true;
+            __syncthreads();
+            const int mine = min(8, rows - n * 8) * D / 4;
+            for (int i = tid; i < mine; i += kAttnThreads) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4, row = n * 8 + r;
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                float most = -INFINITY, weight = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float4 x = *reinterpret_cast<const float4*>(&join[(w * 8 + r) * D + (d ^ ((r >> 1) * 8))]);
+                    sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+                    most = fmaxf(most, s_m[w][row]);
+                }
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) weight = fmaf(s_l[w][row], exp2_approx(s_m[w][row] - finite_ref(most)), weight);
+                if (whole) {
+                    const float inv = weight == 0.f ? 0.f : 1.f / weight;
+                    sum.x *= inv, sum.y *= inv, sum.z *= inv, sum.w *= inv;
+                    *reinterpret_cast<uint2*>(p.out + (head0 + row) * D + d) = pack4<BF16>(sum);
+                    if (d == 0) store_lse(p, head0 + row, weight, most);
+                } else {
+                    *reinterpret_cast<float4*>(part + row * D + d) = sum;
+                    if (d == 0) *reinterpret_cast<float2*>(part + ROWS * D + 2 * row) = make_float2(most, weight);
+                }
+            }
+            __syncthreads();
         }
+        if ((st.last & 1) != 0) break;
+        fresh = true;
+        from_begin = true;
     }
     cp_async_wait<0>();
 }
 
-// Joins the parts of the units that several shares worked on.  CTA (x, y): the unit inside which share x + 1
-// begins, if that is the first border inside the unit, rows y, y + grid.y, ... of it; the warps take the parts in
-// turn.  The maximum over the parts comes first, so that nothing in the loop over the accumulators waits for
-// the part before.
+// Joins the parts of the units that several shares worked on.  CTAs (x, ...) take the unit inside which share x + 1
+// begins, if that is the first border inside the unit.  Up to 32 parts: one warp per row, rows spread over
+// the CTAs (x, y) and their warps; the loads of the accumulators wait for nothing but the unit's place.  More parts
+// (few units, very long): the eight warps of a CTA take every eighth part of a row.
 constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 8;           // rows of a unit that are joined side by side
+constexpr int kJoinRows = 8;           // CTAs (x, y) of a unit, at most
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnParams p, int rows) {
-    constexpr int kJoinWarps = kJoinThreads / 32, V = D / 32;
-    __shared__ float s_o[kJoinWarps][D];
-    pdl_launch_dependents();
-    pdl_wait_prior_grid();
+    constexpr int kJoinWarps = kJoinThreads / 32, V = D / 64;      // pairs of elements of a lane
+    __shared__ float2 s_o[kJoinWarps][D / 2];
+    __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int share = blockIdx.x + 1;
+    pdl_wait_prior_grid();
     const ShareInfo info = p.info[share];
     if (!info.inside) return;
     const int first = share_of(info.unit_begin, info.total, info.shares);
     if (share != first + 1) return;
     const int count = share_of(info.unit_end - 1, info.total, info.shares) - first + 1;
     const int per_request = p.heads_k * p.row_blocks;
-    const int b = info.unit / per_request, u = info.unit % per_request;
-    const int hk = u / p.row_blocks, row0 = (u % p.row_blocks) * rows;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto part = [&](int i) { return p.parts + (2 * static_cast<long long>(first + i) + (i == 0 ? 1 : 0)) * p.part_floats; };
-    for (int row = blockIdx.y; row < rows && row0 + row < p.group; row += gridDim.y) {
-        float top = -INFINITY;
-        for (int i = lane; i < count; i += 32) top = fmaxf(top, part(i)[rows * D + 2 * row]);
+    const int b = info.unit / per_request, u = info.unit - b * per_request;
+    const int hk = u / p.row_blocks, row0 = (u - hk * p.row_blocks) * rows;
+    const long long head0 = static_cast<long long>(b) * p.heads + hk * p.group + row0;
+    const int last_row = min(rows, p.group - row0);
+    const bool together = count > 32;                  // the warps of a CTA work on one row
+    const int step = together ? kJoinWarps : 1;
+    for (int row = blockIdx.y + (together ? 0 : gridDim.y * warp); row < last_row; row += gridDim.y * (together ? 1 : kJoinWarps)) {
+        float top = -INFINITY, sum = 0.f;
+        float2 acc[V];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float ref = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
-        for (int i = lane; i < count; i += 32) {
-            const float* x = part(i) + rows * D + 2 * row;
-            sum = fmaf(exp2_approx(x[0] - ref), x[1], sum);
+        for (int v = 0; v < V; ++v) acc[v] = make_float2(0.f, 0.f);
+        constexpr int U = 4;
+        for (int i0 = together ? warp : 0; i0 < count; i0 += U * step) {
+            float2 ml[U], x[U][V];
+#pragma unroll
+            for (int c = 0; c < U; ++c) {
+                const int i = i0 + c * step;
+                ml[c] = make_float2(-INFINITY, 0.f);
+                if (i < count) {
+                    const float* part = p.parts + (2 * static_cast<long long>(first + i) + (i == 0 ? 1 : 0)) * p.part_floats;
+                    ml[c] = *reinterpret_cast<const float2*>(part + rows * D + 2 * row);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) x[c][v] = *reinterpret_cast<const float2*>(part + row * D + v * 64 + lane * 2);
+                }
+            }
+            float now = top;
+#pragma unroll
+            for (int c = 0; c < U; ++c) now = fmaxf(now, ml[c].x);
+            const float ref = finite_ref(now), f = exp2_approx(top - ref);
+            sum *= f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[v].x *= f, acc[v].y *= f;
+#pragma unroll
+            for (int c = 0; c < U; ++c) {
+                if (i0 + c * step >= count) break;
+                const float g = exp2_approx(ml[c].x - ref);
+                sum = fmaf(g, ml[c].y, sum);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    acc[v].x = fmaf(g, x[c][v].x, acc[v].x);
+                    acc[v].y = fmaf(g, x[c][v].y, acc[v].y);
+                }
+            }
+            top = now;
         }
+        if (together) {
+            if (lane == 0) {
+                s_m[warp] = top;
+                s_l[warp] = sum;
+            }
+            __syncthreads();
+            float most = -INFINITY;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        float acc[V];
+            for (int w = 0; w < kJoinWarps; ++w) most = fmaxf(most, s_m[w]);
+            const float f = exp2_approx(top - finite_ref(most));
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = 0.f;
-#pragma unroll 4
-        for (int i = warp; i < count; i += kJoinWarps) {
-            const float* x = part(i);
-            const float f = exp2_approx(x[rows * D + 2 * row] - ref);
+            for (int v = 0; v < V; ++v) s_o[warp][v * 32 + lane] = make_float2(acc[v].x * f, acc[v].y * f);
+            sum = 0.f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] = fmaf(f, x[row * D + v * 32 + lane], acc[v]);
+            for (int w = 0; w < kJoinWarps; ++w) sum = fmaf(s_l[w], exp2_approx(s_m[w] - finite_ref(most)), sum);
+            top = most;
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                acc[v] = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kJoinWarps; ++w) {
+                    const float2 x = s_o[w][v * 32 + lane];
+                    acc[v].x += x.x, acc[v].y += x.y;
+                }
+            }
+            __syncthreads();
         }
+        if (!together || warp == 0) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int v = 0; v < V; ++v) s_o[warp][v * 32 + lane] = acc[v];
-        __syncthreads();
-        if (tid < D) {
-            float o = 0.f;
-#pragma unroll
-            for (int w = 0; w < kJoinWarps; ++w) o += s_o[w][tid];
-            const long long h = static_cast<long long>(b) * p.heads + hk * p.group + row0 + row;
-            const float v = sum == 0.f ? 0.f : o / sum;
-            p.out[h * D + tid] = static_cast<uint16_t>(pack2<BF16>(v, 0.f));
-            if (tid == 0 && p.lse != nullptr) p.lse[h] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+            for (int v = 0; v < V; ++v)
+                *reinterpret_cast<uint32_t*>(p.out + (head0 + row) * D + v * 64 + lane * 2) = pack2<BF16>(acc[v].x * inv, acc[v].y * inv);
+            if (lane == 0) store_lse(p, head0 + row, sum, top);
         }
-        __syncthreads();
     }
 }
 
@@ -1211,8 +1286,13 @@ static int launch_rotary(const RotaryParams& p, bool interleaved, long long toke
                 : launch_rotary<64, false>(p, interleaved, tokens, outer, sms, stream);
 }
 
+// Key tiles of a unit up to which one CTA does it alone: six to eight tiles of a CTA without company take what
+// one tile, the partial result and the joining kernel take (about 6 us), and a second launch costs the host 2 us.
+constexpr int kWholeTiles = 8;
+
 struct AttnPlan {
     int grid, nt, row_blocks;
+    bool whole;
     long long part_floats;
     size_t info_bytes, bytes;
 };
@@ -1243,11 +1323,20 @@ static int make_attn_plan(const FaPagedAttentionArgs* a, int sms, AttnPlan* plan
     const int group = a->heads / a->cache.heads_k;
     plan->nt = group <= 8 ? 1 : group <= 16 ? 2 : 4;
     plan->row_blocks = (group + plan->nt * 8 - 1) / (plan->nt * 8);
-    const long long tiles = (static_cast<long long>(a->table_width) * a->cache.page_size + attn_tile(D) - 1) / attn_tile(D);
+    const long long capacity = static_cast<long long>(a->table_width) * a->cache.page_size;
+    const long long tiles = (capacity + attn_tile(D) - 1) / attn_tile(D);
     const long long most = static_cast<long long>(a->batch) * a->cache.heads_k * plan->row_blocks * (tiles > 0 ? tiles : 1);
     const long long resident = static_cast<long long>(D == 64 && plan->nt == 1 ? AttnCfg<64, 1>::kCtas : AttnCfg<D, 2>::kCtas) * sms;
     // tiles of one request, and of one share, are counted in 32 bits
     if (tiles * a->cache.heads_k * plan->row_blocks > INT_MAX || most / resident >= INT_MAX) return FA_PAGED_ERR_SHAPE;
+    // with many units, equal shares beat whole units: no last round
+    const long long units = static_cast<long long>(a->batch) * a->cache.heads_k * plan->row_blocks;
+    const long long seen = a->window > 0 && a->window < capacity ? a->window / attn_tile(D) + 2 : tiles;      // of one unit, at most
+    plan->whole = seen <= 1 || (seen <= kWholeTiles && units <= resident);
+    if (plan->whole) {
+        plan->grid = static_cast<int>(units);
+        return FA_PAGED_OK;
+    }
     plan->grid = static_cast<int>(most < resident ? most : resident);
     plan->part_floats = plan->nt * 8 * (D + 2);
     plan->info_bytes = (plan->grid * sizeof(ShareInfo) + 255) / 256 * 256;
@@ -1272,7 +1361,7 @@ static int launch_attention(const AttnParams& p, const AttnPlan& plan, int devic
     int rc = allow_smem(paged_attention_kernel<D, BF16, NT, CAP>, smem, done, device);
     if (rc != FA_PAGED_OK) return rc;
     rc = launch_chained(paged_attention_kernel<D, BF16, NT, CAP>, dim3(plan.grid), kAttnThreads, smem, stream, p);
-    if (rc != FA_PAGED_OK || plan.grid < 2) return rc;
+    if (rc != FA_PAGED_OK || plan.whole) return rc;
     const int rows = p.group < kJoinRows ? p.group : kJoinRows;
     return launch_chained(paged_join_kernel<D, BF16>, dim3(plan.grid - 1, rows), kJoinThreads, 0, stream, p, NT * 8);
 }
@@ -1298,7 +1387,7 @@ static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t byte
     if (rc != FA_PAGED_OK || plan.grid == 0) return rc;
     if (a->q == nullptr || a->out == nullptr || a->lens == nullptr || (a->table_width > 0 && a->block_table == nullptr))
         return FA_PAGED_ERR_NULL;
-    if (workspace == nullptr || bytes < plan.bytes || !aligned16(workspace)) return FA_PAGED_ERR_WORKSPACE;
+    if (plan.bytes > 0 && (workspace == nullptr || bytes < plan.bytes || !aligned16(workspace))) return FA_PAGED_ERR_WORKSPACE;
     DeviceGuard guard(a->device);
     if (guard.err != cudaSuccess) return cuda_failed();
     const FaPagedCache& c = a->cache;
@@ -1325,6 +1414,7 @@ static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t byte
     while ((1LL << s) < c.page_size) ++s;
     p.page_mul = static_cast<unsigned>(((1ULL << (31 + s)) + c.page_size - 1) / c.page_size);
     p.page_shift = 31 + s;
+    p.whole = plan.whole;
     p.info = static_cast<ShareInfo*>(workspace);
     p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.info_bytes);
     p.part_floats = plan.part_floats;

@@ -591,16 +591,15 @@ struct AttnParams {
     // tanh(y) = 1 - 2 / (1 + 2^(2 log2(e) y))
     float scale2, cap2, inner;
     // workspace
-    struct ShareInfo* info;       // one per CTA
+    struct CutInfo* cuts;         // one per unit, or one per CTA where there are more units than CTAs
+    int cuts_by_unit;
     float* parts;                 // two per CTA: rows * D of o, then rows (m, l)
     long long part_floats;
 };
 
-// The unit in which a share begins, if it begins inside one.
-struct ShareInfo {
-    long long unit_begin, unit_end;       // its tiles in the sequence
-    long long total;                      // all tiles of the launch
-    int unit, inside, shares, pad;
+// A unit that is cut in parts: those of `count` shares from `first` on; count = 0: nothing to join.
+struct CutInfo {
+    int unit, first, count, pad;
 };
 
 struct Range {
@@ -673,10 +672,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         __syncthreads();
         const long long total = s_total;
         const int shares = total < gridDim.x ? static_cast<int>(total) : static_cast<int>(gridDim.x);
-        if (share >= shares) {
-            if (tid == 0) p.info[share].inside = 0;
-            return;
-        }
+        if (share >= shares) return;                 // fewer tiles than CTAs, so the cuts are told by unit
         const long long begin = share_begin(share, total, shares);
         to_load = static_cast<int>(share_begin(share + 1, total, shares) - begin);
         if (begin >= upto - mine && begin < upto) {
@@ -701,17 +697,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         const unsigned tiles = lr.tile_hi - lr.tile_lo;
         lu = off / tiles;
         lt = lr.tile_lo + off - lu * tiles;
-        if (tid == 0) {
-            ShareInfo info;
-            info.unit_begin = s_at + static_cast<long long>(lu) * tiles;
-            info.unit_end = info.unit_begin + tiles;
-            info.total = total;
-            info.unit = lb * per_request + lu;
-            info.inside = info.unit_begin < begin;
-            info.shares = shares;
-            info.pad = 0;
-            p.info[share] = info;
-        }
     }
     bool from_begin = lt == lr.tile_lo;              // this part of a unit contains its first key
 
@@ -1043,6 +1028,17 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
             }
             __syncthreads();
         }
+        if (tid == 0 && !p.whole && (p.cuts_by_unit ? from_begin : (st.last & 1) != 0)) {
+            CutInfo cut{st.b * per_request + st.unit, share, 0, 0};
+            if (from_begin && !whole) {              // the last part here: it ends with the share
+                const Range r = key_range<C::kTile>(p, p.lens[st.b]);
+                const int shares = s_total < gridDim.x ? static_cast<int>(s_total) : static_cast<int>(gridDim.x);
+                const int done = (st.rel + r.hi - 1) / C::kTile - r.tile_lo + 1;
+                const long long unit_end = share_begin(share + 1, s_total, shares) - done + (r.tile_hi - r.tile_lo);
+                cut.count = share_of(unit_end - 1, s_total, shares) - share + 1;
+            }
+            p.cuts[p.cuts_by_unit ? cut.unit : share] = cut;
+        }
         if ((st.last & 1) != 0) break;
         fresh = true;
         from_begin = true;
@@ -1050,108 +1046,89 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     cp_async_wait<0>();
 }
 
-// Joins the parts of the units that several shares worked on.  CTAs (x, ...) take the unit inside which share x + 1
-// begins, if that is the first border inside the unit.  Up to 32 parts: one warp per row, rows spread over
-// the CTAs (x, y) and their warps; the loads of the accumulators wait for nothing but the unit's place.  More parts
-// (few units, very long): the eight warps of a CTA take every eighth part of a row.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 8;           // CTAs (x, y) of a unit, at most
+// Joins the parts of the units that several shares worked on.  CTA (x, y): the unit of cut x, rows from
+// y * rows_per_cta on; the CTA's warps are shared out evenly among its rows, take a row's parts in turn, four at a time
+// with all their loads in flight, and are joined through shared memory.
+constexpr int kJoinThreads = 512;      // at most
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnParams p, int rows) {
-    constexpr int kJoinWarps = kJoinThreads / 32, V = D / 64;      // pairs of elements of a lane
+__global__ void __launch_bounds__(kJoinThreads, 2) paged_join_kernel(const AttnParams p, int rows, int rows_per_cta) {
+    constexpr int kJoinWarps = kJoinThreads / 32, V = D / 64, U = 4;      // V: pairs of elements of a lane
     __shared__ float2 s_o[kJoinWarps][D / 2];
     __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int share = blockIdx.x + 1;
+    const int team = static_cast<int>(blockDim.x / 32) / rows_per_cta, member = warp % team, row = blockIdx.y * rows_per_cta + warp / team;
     pdl_wait_prior_grid();
-    const ShareInfo info = p.info[share];
-    if (!info.inside) return;
-    const int first = share_of(info.unit_begin, info.total, info.shares);
-    if (share != first + 1) return;
-    const int count = share_of(info.unit_end - 1, info.total, info.shares) - first + 1;
-    const int per_request = p.heads_k * p.row_blocks;
-    const int b = info.unit / per_request, u = info.unit - b * per_request;
-    const int hk = u / p.row_blocks, row0 = (u - hk * p.row_blocks) * rows;
-    const long long head0 = static_cast<long long>(b) * p.heads + hk * p.group + row0;
-    const int last_row = min(rows, p.group - row0);
-    const bool together = count > 32;                  // the warps of a CTA work on one row
-    const int step = together ? kJoinWarps : 1;
-    for (int row = blockIdx.y + (together ? 0 : gridDim.y * warp); row < last_row; row += gridDim.y * (together ? 1 : kJoinWarps)) {
-        float top = -INFINITY, sum = 0.f;
-        float2 acc[V];
+    const int4 cut = *reinterpret_cast<const int4*>(p.cuts + blockIdx.x);
+    const int count = cut.z;
+    if (count == 0) return;
+    float top = -INFINITY, sum = 0.f;
+    float2 acc[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = make_float2(0.f, 0.f);
-        constexpr int U = 4;
-        for (int i0 = together ? warp : 0; i0 < count; i0 += U * step) {
-            float2 ml[U], x[U][V];
+    for (int v = 0; v < V; ++v) acc[v] = make_float2(0.f, 0.f);
+    // (a row behind the group's last holds nothing, and is not stored below)
+    for (int i0 = member; i0 < count; i0 += U * team) {
+        float2 ml[U], x[U][V];
 #pragma unroll
-            for (int c = 0; c < U; ++c) {
-                const int i = i0 + c * step;
-                ml[c] = make_float2(-INFINITY, 0.f);
-                if (i < count) {
-                    const float* part = p.parts + (2 * static_cast<long long>(first + i) + (i == 0 ? 1 : 0)) * p.part_floats;
-                    ml[c] = *reinterpret_cast<const float2*>(part + rows * D + 2 * row);
+        for (int c = 0; c < U; ++c) {
+            const int i = i0 + c * team;
+            ml[c] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) x[c][v] = *reinterpret_cast<const float2*>(part + row * D + v * 64 + lane * 2);
-                }
+            for (int v = 0; v < V; ++v) x[c][v] = make_float2(0.f, 0.f);
+            if (i < count && row < rows) {
+                const float* part = p.parts + (2 * static_cast<long long>(cut.y + i) + (i == 0 ? 1 : 0)) * p.part_floats;
+                ml[c] = *reinterpret_cast<const float2*>(part + rows * D + 2 * row);
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[c][v] = *reinterpret_cast<const float2*>(part + row * D + v * 64 + lane * 2);
             }
-            float now = top;
-#pragma unroll
-            for (int c = 0; c < U; ++c) now = fmaxf(now, ml[c].x);
-            const float ref = finite_ref(now), f = exp2_approx(top - ref);
-            sum *= f;
-#pragma unroll
-            for (int v = 0; v < V; ++v) acc[v].x *= f, acc[v].y *= f;
-#pragma unroll
-            for (int c = 0; c < U; ++c) {
-                if (i0 + c * step >= count) break;
-                const float g = exp2_approx(ml[c].x - ref);
-                sum = fmaf(g, ml[c].y, sum);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    acc[v].x = fmaf(g, x[c][v].x, acc[v].x);
-                    acc[v].y = fmaf(g, x[c][v].y, acc[v].y);
-                }
-            }
-            top = now;
         }
-        if (together) {
-            if (lane == 0) {
-                s_m[warp] = top;
-                s_l[warp] = sum;
-            }
-            __syncthreads();
-            float most = -INFINITY;
+        float now = top;
 #pragma unroll
-            for (int w = 0; w < kJoinWarps; ++w) most = fmaxf(most, s_m[w]);
-            const float f = exp2_approx(top - finite_ref(most));
+        for (int c = 0; c < U; ++c) now = fmaxf(now, ml[c].x);
+        const float ref = finite_ref(now), f = exp2_approx(top - ref);
+        sum *= f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) s_o[warp][v * 32 + lane] = make_float2(acc[v].x * f, acc[v].y * f);
-            sum = 0.f;
+        for (int v = 0; v < V; ++v) acc[v].x *= f, acc[v].y *= f;
 #pragma unroll
-            for (int w = 0; w < kJoinWarps; ++w) sum = fmaf(s_l[w], exp2_approx(s_m[w] - finite_ref(most)), sum);
-            top = most;
-            __syncthreads();
+        for (int c = 0; c < U; ++c) {
+            const float g = exp2_approx(ml[c].x - ref);
+            sum = fmaf(g, ml[c].y, sum);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                acc[v] = make_float2(0.f, 0.f);
-#pragma unroll
-                for (int w = 0; w < kJoinWarps; ++w) {
-                    const float2 x = s_o[w][v * 32 + lane];
-                    acc[v].x += x.x, acc[v].y += x.y;
-                }
+                acc[v].x = fmaf(g, x[c][v].x, acc[v].x);
+                acc[v].y = fmaf(g, x[c][v].y, acc[v].y);
             }
-            __syncthreads();
         }
-        if (!together || warp == 0) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                *reinterpret_cast<uint32_t*>(p.out + (head0 + row) * D + v * 64 + lane * 2) = pack2<BF16>(acc[v].x * inv, acc[v].y * inv);
-            if (lane == 0) store_lse(p, head0 + row, sum, top);
-        }
+        top = now;
     }
+    if (lane == 0) {
+        s_m[warp] = top;
+        s_l[warp] = sum;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_o[warp][v * 32 + lane] = acc[v];
+    __syncthreads();
+    const int per_request = p.heads_k * p.row_blocks;
+    const int b = cut.x / per_request, u = cut.x - b * per_request, hk = u / p.row_blocks, row0 = (u - hk * p.row_blocks) * rows;
+    if (member != 0 || row >= rows || row0 + row >= p.group) return;
+    for (int w = 1; w < team; ++w) {
+        const float now = fmaxf(top, s_m[warp + w]), ref = finite_ref(now);
+        const float f = exp2_approx(top - ref), g = exp2_approx(s_m[warp + w] - ref);
+        sum = sum * f + s_l[warp + w] * g;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const float2 x = s_o[warp + w][v * 32 + lane];
+            acc[v].x = acc[v].x * f + x.x * g;
+            acc[v].y = acc[v].y * f + x.y * g;
+        }
+        top = now;
+    }
+    const long long head = static_cast<long long>(b) * p.heads + hk * p.group + row0 + row;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+        *reinterpret_cast<uint32_t*>(p.out + head * D + v * 64 + lane * 2) = pack2<BF16>(acc[v].x * inv, acc[v].y * inv);
+    if (lane == 0) store_lse(p, head, sum, top);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1294,7 +1271,8 @@ struct AttnPlan {
     int grid, nt, row_blocks;
     bool whole;
     long long part_floats;
-    size_t info_bytes, bytes;
+    int cuts, rows_per_cta, join_warps;       // of the joining kernel
+    size_t cut_bytes, bytes;
 };
 
 static int check_attention(const FaPagedAttentionArgs* a) {
@@ -1339,8 +1317,22 @@ static int make_attn_plan(const FaPagedAttentionArgs* a, int sms, AttnPlan* plan
     }
     plan->grid = static_cast<int>(most < resident ? most : resident);
     plan->part_floats = plan->nt * 8 * (D + 2);
-    plan->info_bytes = (plan->grid * sizeof(ShareInfo) + 255) / 256 * 256;
-    plan->bytes = plan->info_bytes + 2 * plan->grid * plan->part_floats * sizeof(float);
+    plan->cuts = static_cast<int>(units < plan->grid ? units : plan->grid);
+    // Few parts per unit: one CTA does all rows (up to 16) with eight warps at most.  Many: sixteen warps, and a CTA per
+    // row as long as they all run at once, four to an SM.  (Sixteen warps a row cost 32 requests of 8 KV heads 0.5 us
+    // and 768 units of one row 2.5; four parts a warp are one round of loads.)
+    const int rows = group < plan->nt * 8 ? group : plan->nt * 8;
+    plan->rows_per_cta = 1;
+    if (plan->grid / units < 4) {
+        while (plan->rows_per_cta < 16 && plan->rows_per_cta < rows) plan->rows_per_cta *= 2;
+        plan->join_warps = plan->rows_per_cta == 1 ? 4 : plan->rows_per_cta <= 8 ? 8 : 16;
+    } else {
+        while (plan->rows_per_cta < 16 && static_cast<long long>(plan->cuts) * ((rows + plan->rows_per_cta - 1) / plan->rows_per_cta) > 4LL * sms)
+            plan->rows_per_cta *= 2;
+        plan->join_warps = 16;
+    }
+    plan->cut_bytes = (plan->cuts * sizeof(CutInfo) + 255) / 256 * 256;
+    plan->bytes = plan->cut_bytes + 2 * plan->grid * plan->part_floats * sizeof(float);
     return FA_PAGED_OK;
 }
 
@@ -1362,8 +1354,9 @@ static int launch_attention(const AttnParams& p, const AttnPlan& plan, int devic
     if (rc != FA_PAGED_OK) return rc;
     rc = launch_chained(paged_attention_kernel<D, BF16, NT, CAP>, dim3(plan.grid), kAttnThreads, smem, stream, p);
     if (rc != FA_PAGED_OK || plan.whole) return rc;
-    const int rows = p.group < kJoinRows ? p.group : kJoinRows;
-    return launch_chained(paged_join_kernel<D, BF16>, dim3(plan.grid - 1, rows), kJoinThreads, 0, stream, p, NT * 8);
+    const int rows = p.group < NT * 8 ? p.group : NT * 8;
+    const dim3 grid(plan.cuts, (rows + plan.rows_per_cta - 1) / plan.rows_per_cta);
+    return launch_chained(paged_join_kernel<D, BF16>, grid, plan.join_warps * 32, 0, stream, p, NT * 8, plan.rows_per_cta);
 }
 
 template <int D, bool BF16, int NT>
@@ -1415,8 +1408,9 @@ static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t byte
     p.page_mul = static_cast<unsigned>(((1ULL << (31 + s)) + c.page_size - 1) / c.page_size);
     p.page_shift = 31 + s;
     p.whole = plan.whole;
-    p.info = static_cast<ShareInfo*>(workspace);
-    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.info_bytes);
+    p.cuts = static_cast<CutInfo*>(workspace);
+    p.cuts_by_unit = plan.cuts < plan.grid || plan.whole;
+    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.cut_bytes);
     p.part_floats = plan.part_floats;
     const bool bf16 = a->dtype == FA_PAGED_BF16;
     if (c.head_dim == 128)

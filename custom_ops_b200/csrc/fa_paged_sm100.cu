@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const Shrin
 // are worked out.  Tokens per CTA: as many as keep a thread at kRotaryBatch heads at most, so that all of a CTA's
 // loads are in flight together - unless that leaves SMs without a CTA.
 constexpr int kRotaryThreads = 128;
-constexpr int kRotaryBatch = 4;
+constexpr int kRotaryBatch = 3;
 constexpr int kRotaryTokens = 8;
 constexpr int kRotaryWaves = 4;       // CTAs per SM that there have to be
 
@@ -393,7 +393,6 @@ enum Pairing {
 template <int D, bool BF16, int PAIRING>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p) {
     __shared__ __align__(16) float2 s_turn[kRotaryTokens * D / 2];     // (cos, sin) * mscale of each pair
-    pdl_launch_dependents();
     const int tid = threadIdx.x;
     constexpr int kParts = D / 16;
     const int part = tid % kParts, mine = tid / kParts % p.per_cta, start = tid / kParts / p.per_cta;

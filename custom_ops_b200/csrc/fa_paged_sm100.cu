@@ -50,6 +50,22 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// The address of another cluster CTA's copy of a shared-memory location, and loads from there.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -527,7 +543,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
 //
 // Bound: memory.  A key of a KV head costs 4 * head_dim bytes and 4 * head_dim flops per query head of the
 // group, so even 32 heads a group stay far from the tensor pipe's balance (250 flops a byte).  What matters is
-// to keep enough loads in flight on every SM, whatever the lengths are.
+// to keep enough loads in flight on every SM, whatever the lengths are, and, for short histories, that little has to
+// happen one after the other.
 //
 // Work: the requests' key ranges, per KV head, are cut in tiles of kTile keys and laid one behind the other -
 // request, then KV head, then row block, then tile - and every CTA takes an equal, consecutive share of that
@@ -584,7 +601,7 @@ struct AttnParams {
     long long q_batch, q_head, table_stride;
     long long k_page, k_head, k_row, v_page, v_head, v_row;
     int batch, heads, heads_k, group, row_blocks, width, page_size, num_pages, window;
-    int whole;                    // 1: CTA u does unit u from its first key to its last
+    int cluster;                  // n > 0: unit u is done by the n CTAs from n u on, a cluster; 0: equal shares
     unsigned page_mul, page_shift;      // key / page_size = key * page_mul >> page_shift, for keys below 2^31
     // x, in powers of two, is s * scale2, or with a cap  cap2 * tanh(s * inner / 2),  inner = 2 log2(e) scale / cap:
     // tanh(y) = 1 - 2 / (1 + 2^(2 log2(e) y))
@@ -634,6 +651,41 @@ __device__ __forceinline__ void store_lse(const AttnParams& p, long long head, f
     if (p.lse != nullptr) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
+// Joins the parts that the CTAs of a cluster have in their shared memory: rows * D of o, then rows (m, l).  Every CTA
+// takes its share of the elements and reads all the parts.
+template <int D, bool BF16, int ROWS>
+__device__ __forceinline__ void join_cluster(const AttnParams& p, const float* part) {
+    const int tid = threadIdx.x, rank = static_cast<int>(cluster_rank()), unit = blockIdx.x / p.cluster;
+    const int per_request = p.heads_k * p.row_blocks;
+    const int b = unit / per_request, u = unit - b * per_request, hk = u / p.row_blocks, row0 = (u - hk * p.row_blocks) * ROWS;
+    const int rows = min(ROWS, p.group - row0);
+    const long long head0 = static_cast<long long>(b) * p.heads + hk * p.group + row0;
+    const uint32_t mine = smem_u32(part);
+    cluster_arrive();
+    cluster_wait();                  // the parts are there
+    for (int i = (rank * kAttnThreads + tid) * 4; i < rows * D; i += p.cluster * kAttnThreads * 4) {
+        const int row = i / D;
+        float top = -INFINITY, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < p.cluster; ++c) {
+            const uint32_t theirs = cluster_addr(mine, c);
+            const float2 ml = ld_cluster_v2(theirs + (ROWS * D + 2 * row) * 4);
+            if (ml.y == 0.f) continue;                   // nothing seen; its o may never have been written
+            const float4 x = ld_cluster_v4(theirs + i * 4);
+            const float now = fmaxf(top, ml.x), f = exp2_approx(top - now), g = exp2_approx(ml.x - now);
+            sum = sum * f + ml.y * g;
+            acc.x = acc.x * f + x.x * g, acc.y = acc.y * f + x.y * g, acc.z = acc.z * f + x.z * g, acc.w = acc.w * f + x.w * g;
+            top = now;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+        *reinterpret_cast<uint2*>(p.out + head0 * D + i) = pack4<BF16>(acc);
+        if (i % D == 0) store_lse(p, head0 + row, sum, top);
+    }
+    cluster_arrive();
+    cluster_wait();                  // and have been read
+}
+
 template <int D, bool BF16, int NT, bool CAP>
 __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_attention_kernel(const AttnParams p) {
     using C = AttnCfg<D, NT>;
@@ -652,12 +704,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     // ---- my share; the loader's place: request, unit within the request, tile
     int lb, lu, lt, to_load;
     Range lr;
-    if (p.whole) {
-        lb = share / per_request;
-        lu = share - lb * per_request;
+    if (p.cluster > 0) {
+        const int rank = static_cast<int>(cluster_rank()), unit = share / p.cluster;
+        lb = unit / per_request;
+        lu = unit - lb * per_request;
         lr = key_range<C::kTile>(p, p.lens[lb]);
-        lt = lr.tile_lo;
-        to_load = lr.tile_hi - lt;
+        const int tiles = lr.tile_hi - lr.tile_lo;       // 8 CTAs at most, of kUnitTiles tiles
+        lt = lr.tile_lo + tiles * rank / p.cluster;
+        to_load = lr.tile_lo + tiles * (rank + 1) / p.cluster - lt;
     } else {
         const int chunk = (p.batch + kAttnThreads - 1) / kAttnThreads;
         const int b_lo = min(tid * chunk, p.batch), b_hi = min(b_lo + chunk, p.batch);
@@ -723,6 +777,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     };
     look_up();
 
+    if (to_load == 0) {                              // a cluster that has more CTAs than the unit tiles
+        for (int r = tid; r < ROWS; r += kAttnThreads)
+            *reinterpret_cast<float2*>(s_ring + (ROWS * D + 2 * r) * 4) = make_float2(-INFINITY, 0.f);
+        join_cluster<D, BF16, ROWS>(p, reinterpret_cast<const float*>(s_ring));
+        return;
+    }
     float o[DT][NT][4], m[NT][2], l[NT][2];
     uint32_t qf[C::kQueryInSmem ? 1 : NT][C::kQueryInSmem ? 1 : KK][2];
     bool fresh = true;               // a unit begins
@@ -968,10 +1028,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
 
         // ---- the unit ends, or the share does: the four warps' results become one.  Each warp scales its own to the
         // maximum of the four; what is left is a sum, eight heads at a time through shared memory.
-        const bool whole = from_begin && (st.last & 2) != 0;
+        const bool whole = p.cluster <= 1 && from_begin && (st.last & 2) != 0;
         const int rows = min(p.group - row0, ROWS);
         const long long head0 = static_cast<long long>(st.b) * p.heads + hk * p.group + row0;
-        float* const part = p.parts + (2 * static_cast<long long>(share) + (from_begin ? 1 : 0)) * p.part_floats;
+        // a cluster's parts stay in shared memory, where the loads, all done, have been
+        float* const part = p.cluster > 1 ? reinterpret_cast<float*>(s_ring)
+                                          : p.parts + (2 * static_cast<long long>(share) + (from_begin ? 1 : 0)) * p.part_floats;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1027,7 +1089,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
             }
             __syncthreads();
         }
-        if (tid == 0 && !p.whole && (p.cuts_by_unit ? from_begin : (st.last & 1) != 0)) {
+        if (tid == 0 && p.cluster == 0 && (p.cuts_by_unit ? from_begin : (st.last & 1) != 0)) {
             CutInfo cut{st.b * per_request + st.unit, share, 0, 0};
             if (from_begin && !whole) {              // the last part here: it ends with the share
                 const Range r = key_range<C::kTile>(p, p.lens[st.b]);
@@ -1043,6 +1105,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         from_begin = true;
     }
     cp_async_wait<0>();
+    if (p.cluster > 1) join_cluster<D, BF16, ROWS>(p, reinterpret_cast<const float*>(s_ring));
 }
 
 // Joins the parts of the units that several shares worked on.  CTA (x, y): the unit of cut x, rows from
@@ -1262,13 +1325,15 @@ static int launch_rotary(const RotaryParams& p, bool interleaved, long long toke
                 : launch_rotary<64, false>(p, interleaved, tokens, outer, sms, stream);
 }
 
-// Key tiles of a unit up to which one CTA does it alone: six to eight tiles of a CTA without company take what
-// one tile, the partial result and the joining kernel take (about 6 us), and a second launch costs the host 2 us.
-constexpr int kWholeTiles = 8;
+// Short units: each is done by a cluster of 1 to 8 CTAs that join their parts through their shared memory.  No sums
+// over the lengths, no partial results in memory, no second kernel (which costs the host 2 us, too).  Up to so many
+// tiles for a CTA, as long as the CTAs all run at once; with more, equal shares of all keys pay for what they take.
+constexpr int kUnitTiles = 8;
+constexpr int kMostCluster = 8;
 
 struct AttnPlan {
     int grid, nt, row_blocks;
-    bool whole;
+    int cluster;
     long long part_floats;
     int cuts, rows_per_cta, join_warps;       // of the joining kernel
     size_t cut_bytes, bytes;
@@ -1309,9 +1374,11 @@ static int make_attn_plan(const FaPagedAttentionArgs* a, int sms, AttnPlan* plan
     // with many units, equal shares beat whole units: no last round
     const long long units = static_cast<long long>(a->batch) * a->cache.heads_k * plan->row_blocks;
     const long long seen = a->window > 0 && a->window < capacity ? a->window / attn_tile(D) + 2 : tiles;      // of one unit, at most
-    plan->whole = seen <= 1 || (seen <= kWholeTiles && units <= resident);
-    if (plan->whole) {
-        plan->grid = static_cast<int>(units);
+    int cluster = 1;
+    while (cluster < kMostCluster && 2 * cluster <= seen && 2 * cluster * units <= resident) cluster *= 2;
+    if (seen <= 1 || (seen <= static_cast<long long>(kUnitTiles) * cluster && units * cluster <= resident)) {
+        plan->cluster = cluster;
+        plan->grid = static_cast<int>(units * cluster);
         return FA_PAGED_OK;
     }
     plan->grid = static_cast<int>(most < resident ? most : resident);
@@ -1351,8 +1418,8 @@ static int launch_attention(const AttnParams& p, const AttnPlan& plan, int devic
     constexpr int smem = AttnCfg<D, NT>::kSmem;
     int rc = allow_smem(paged_attention_kernel<D, BF16, NT, CAP>, smem, done, device);
     if (rc != FA_PAGED_OK) return rc;
-    rc = launch_chained(paged_attention_kernel<D, BF16, NT, CAP>, dim3(plan.grid), kAttnThreads, smem, stream, p);
-    if (rc != FA_PAGED_OK || plan.whole) return rc;
+    rc = launch_cluster(paged_attention_kernel<D, BF16, NT, CAP>, dim3(plan.grid), kAttnThreads, smem, plan.cluster, stream, p);
+    if (rc != FA_PAGED_OK || plan.cluster > 0) return rc;
     const int rows = p.group < NT * 8 ? p.group : NT * 8;
     const dim3 grid(plan.cuts, (rows + plan.rows_per_cta - 1) / plan.rows_per_cta);
     return launch_chained(paged_join_kernel<D, BF16>, grid, plan.join_warps * 32, 0, stream, p, NT * 8, plan.rows_per_cta);
@@ -1406,9 +1473,9 @@ static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t byte
     while ((1LL << s) < c.page_size) ++s;
     p.page_mul = static_cast<unsigned>(((1ULL << (31 + s)) + c.page_size - 1) / c.page_size);
     p.page_shift = 31 + s;
-    p.whole = plan.whole;
+    p.cluster = plan.cluster;
     p.cuts = static_cast<CutInfo*>(workspace);
-    p.cuts_by_unit = plan.cuts < plan.grid || plan.whole;
+    p.cuts_by_unit = plan.cuts < plan.grid;
     p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.cut_bytes);
     p.part_floats = plan.part_floats;
     const bool bf16 = a->dtype == FA_PAGED_BF16;

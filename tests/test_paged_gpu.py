@@ -151,6 +151,32 @@ def test_attention_split_over_the_gpu(B, H, Hk, d, length):
         assert torch.equal(ops.paged_attention(*args), got)
 
 
+@pytest.mark.parametrize("d,H,Hk", [(128, 8, 2), (64, 3, 3), (128, 32, 1), (64, 24, 2)])
+def test_attention_of_few_short_requests(d, H, Hk):
+    """Few units of few tiles, whatever the table could hold: every way of dividing them up."""
+    tile = 8192 // d
+    for columns in (1, 2, 3, 5, 8, 9, 17, 33, 64, 65):
+        for B in (1, 3, 20):
+            r = random.Random(columns + B)
+            lens = [columns * tile] + [r.choice((0, 1, r.randint(0, columns * tile))) for _ in range(B - 1)]
+            args = make_cache(lens, H=H, Hk=Hk, d=d, page_size=tile, dtype=torch.bfloat16, gen=gen(columns), width=columns)
+            attend_and_check(*args, what=f"{columns} columns, {B} requests")
+            attend_and_check(*args, what=f"{columns} columns, {B} requests", window=tile + 3)
+
+
+def test_attention_passes_nan_on():
+    """A NaN that a row may see is its result, in every way of dividing the work up; other rows are untouched."""
+    for length in (40, 700, 9000):
+        q, k, v, table, lens = make_cache([length, 50], H=4, Hk=2, d=64, page_size=16, dtype=torch.float16, gen=gen(1))
+        want = ops.paged_attention(q, k, v, table, lens)
+        q[0, 1, 5] = float("nan")
+        out, lse = ops.paged_attention_lse(q, k, v, table, lens)
+        assert out[0, 1].isnan().all() and lse[0, 1].isnan()
+        keep = torch.ones(2, 4, dtype=torch.bool)
+        keep[0, 1] = False
+        assert torch.equal(out[keep.cuda()], want[keep.cuda()])
+
+
 def test_attention_of_each_request_alone():
     """A request's result does not depend on its neighbours beyond where its keys are cut."""
     q, k, v, table, lens = make_cache([2000, 17, 640, 0, 333], H=8, Hk=2, d=128, page_size=16, dtype=torch.float16, gen=gen(2))

@@ -142,6 +142,32 @@ __device__ __forceinline__ long long block_scan(long long v, long long* scratch)
     return v + before;
 }
 
+// The same of two values at once.
+__device__ __forceinline__ void block_scan2(long long& a, long long& b, long long (*scratch)[32]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+        if (lane >= o) {
+            a += x;
+            b += y;
+        }
+    }
+    if (lane == 31) {
+        scratch[0][warp] = a;
+        scratch[1][warp] = b;
+    }
+    __syncthreads();
+    long long x = lane < warp && lane < warps ? scratch[0][lane] : 0, y = lane < warp && lane < warps ? scratch[1][lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    a += x;
+    b += y;
+}
+
 // ------------------------------------------------------------------------------------------------
 // Tables from request lengths
 // ------------------------------------------------------------------------------------------------
@@ -152,7 +178,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* scratch)
 // of which works out the (cheap) sums for itself and takes an eighth of the tokens and pages.  A cluster and not
 // a grid, because lens and free_head may be updated in place: they are written behind a cluster barrier, when
 // every CTA has read them.
-constexpr int kTableThreads = 512;
+constexpr int kTableThreads = 512, kTableClusterThreads = 1024;      // of the one CTA, of each of the eight
 constexpr int kTableCluster = 8;
 constexpr long long kTableTokens = 4096;
 
@@ -190,7 +216,7 @@ __device__ __forceinline__ unsigned pages_of(unsigned tokens, unsigned page_size
     return tokens / page_size + (tokens % page_size != 0);
 }
 
-__global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const ExtendParams p) {
+__global__ void __launch_bounds__(kTableClusterThreads) paged_extend_kernel(const ExtendParams p) {
     extern __shared__ int s_table[];
     int* s_cu = s_table;                    // batch + 1: first token of each request
     int* s_len = s_cu + p.batch + 1;        // batch: length before
@@ -199,7 +225,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
     __shared__ long long s_before[2];
     __shared__ int s_head;
     pdl_launch_dependents();
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, threads = blockDim.x;
     const unsigned rank = cluster_rank(), ranks = cluster_size();
     pdl_wait_prior_grid();
     const int head = min(max(p.free_head[0], 0), p.num_free);
@@ -210,15 +236,17 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
         s_before[0] = s_before[1] = 0;
     }
     __syncthreads();
-    for (int base = 0; base < p.batch; base += kTableThreads) {
+    for (int base = 0; base < p.batch; base += threads) {
         const int b = base + tid;
         const bool in = b < p.batch;
         const unsigned len = in ? max(p.lens[b], 0) : 0, add = in ? max(p.new_lens[b], 0) : 0;
         const unsigned have = pages_of(len, p.page_size), want = pages_of(len + add, p.page_size);
         const bool fits = want <= static_cast<unsigned>(p.width);
         const unsigned need = fits ? want - have : 0;
-        const long long tokens = s_before[0] + block_scan(add, s_scan[0]);
-        const long long pages = s_before[1] + block_scan(need, s_scan[1]);
+        long long tokens = add, pages = need;
+        block_scan2(tokens, pages, s_scan);
+        tokens += s_before[0];
+        pages += s_before[1];
         const bool granted = fits && (need == 0 || pages <= avail);
         if (in) {
             s_cu[b + 1] = static_cast<int>(min(tokens, static_cast<long long>(INT_MAX)));
@@ -229,7 +257,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
         const int given = __reduce_max_sync(0xffffffffu, in && granted && need > 0 ? head + static_cast<int>(pages) : 0);
         if ((tid & 31) == 0 && given > 0) atomicMax(&s_head, given);
         __syncthreads();
-        if (tid == kTableThreads - 1) {
+        if (tid == threads - 1) {
             s_before[0] = tokens;
             s_before[1] = pages;
         }
@@ -238,8 +266,8 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
     cluster_arrive();                       // lens and free_head have been read
     const unsigned page_size = p.page_size;
     // new pages: one warp per request
-    const int warps = ranks * (kTableThreads / 32);
-    for (int b = rank * (kTableThreads / 32) + (tid >> 5); b < p.batch; b += warps) {
+    const int warps = ranks * (threads / 32);
+    for (int b = rank * (threads / 32) + (tid >> 5); b < p.batch; b += warps) {
         if (s_src[b] < 0) continue;
         const unsigned len = s_len[b], add = s_cu[b + 1] - s_cu[b];      // len + add: countable in 31 bits, or refused
         const int have = pages_of(len, page_size), want = pages_of(len + add, page_size);
@@ -249,8 +277,8 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
     // slots and positions; a page that is new is read from the free list, not from the row just written
     const long long total = s_cu[p.batch];
     const bool vec = ((reinterpret_cast<uintptr_t>(p.slots) | reinterpret_cast<uintptr_t>(p.positions)) & 15u) == 0;
-    for (long long t0 = 4 * (static_cast<long long>(rank) * kTableThreads + tid); t0 < p.num_tokens;
-         t0 += 4LL * ranks * kTableThreads) {
+    for (long long t0 = 4 * (static_cast<long long>(rank) * threads + tid); t0 < p.num_tokens;
+         t0 += 4LL * ranks * threads) {
         const int* from[4];                              // where the page of each token is named
         unsigned row[4];
         int pos[4];
@@ -297,7 +325,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_extend_kernel(const Exten
         }
     }
     cluster_wait();
-    for (int b = rank * kTableThreads + tid; b < p.batch; b += ranks * kTableThreads) {
+    for (int b = rank * threads + tid; b < p.batch; b += ranks * threads) {
         p.cu[b + 1] = s_cu[b + 1];
         p.lens_out[b] = s_len[b] + (s_src[b] >= 0 ? s_cu[b + 1] - s_cu[b] : 0);
     }
@@ -1605,7 +1633,7 @@ static int extend(const FaPagedExtendArgs* a, cudaStream_t stream) {
     p.batch = a->batch, p.width = a->table_width, p.page_size = a->page_size, p.num_free = a->num_free_pages;
     p.num_tokens = a->num_tokens;
     const int ctas = a->num_tokens >= kTableTokens ? kTableCluster : 1;
-    return launch_cluster(paged_extend_kernel, dim3(ctas), kTableThreads, (3 * static_cast<size_t>(a->batch) + 1) * 4, ctas,
+    return launch_cluster(paged_extend_kernel, dim3(ctas), ctas > 1 ? kTableClusterThreads : kTableThreads, (3 * static_cast<size_t>(a->batch) + 1) * 4, ctas,
                           stream, p);
 }
 

@@ -596,11 +596,13 @@ class RecsysOps:
 
     # ---- the paged key/value cache (no counterpart in the reference)
     def _paged_call(self, backend, name: str):
-        """``_dispatch`` for calls of a few microseconds: the operator is looked up once."""
-        _resolve_backend(backend)
-        op = self._paged_ops.get(name)
+        """``_dispatch`` for calls of a few microseconds: without an explicit backend the operator is looked up,
+        and the environment asked, the first time only."""
+        op = self._paged_ops.get(name) if backend is None else None
         if op is None:
-            op = self._paged_ops[name] = getattr(self._dispatch(backend, "paged"), name).default
+            op = getattr(self._dispatch(backend, "paged"), name).default
+            if backend is None:
+                self._paged_ops[name] = op
         return op
 
     def paged_extend(self, block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,

@@ -741,40 +741,67 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         lt = lr.tile_lo + tiles * rank / p.cluster;
         to_load = lr.tile_lo + tiles * (rank + 1) / p.cluster - lt;
     } else {
-        const int chunk = (p.batch + kAttnThreads - 1) / kAttnThreads;
-        const int b_lo = min(tid * chunk, p.batch), b_hi = min(b_lo + chunk, p.batch);
-        long long mine = 0;
-        for (int b = b_lo; b < b_hi; ++b) {
-            const Range r = key_range<C::kTile>(p, p.lens[b]);
-            mine += static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
-        }
-        const long long upto = block_scan(mine, s_scan);
-        if (tid == kAttnThreads - 1) s_total = upto;
-        __syncthreads();
-        const long long total = s_total;
-        const int shares = total < gridDim.x ? static_cast<int>(total) : static_cast<int>(gridDim.x);
-        if (share >= shares) return;                 // fewer tiles than CTAs, so the cuts are told by unit
-        const long long begin = share_begin(share, total, shares);
-        to_load = static_cast<int>(share_begin(share + 1, total, shares) - begin);
-        if (begin >= upto - mine && begin < upto) {
-            long long at = upto - mine;
-            for (int b = b_lo; b < b_hi; ++b) {
-                const int len = p.lens[b];
-                const Range r = key_range<C::kTile>(p, len);
-                const long long n = static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
-                if (begin < at + n) {
-                    s_request = b;
-                    s_len = len;
-                    s_at = at;
-                    break;
-                }
-                at += n;
+        long long total, begin, at = 0;              // at: the request's first tile in the sequence
+        int len;
+        if (p.batch <= 32) {
+            // every warp by itself: a request per lane, no barrier
+            len = lane < p.batch ? p.lens[lane] : 0;
+            const Range r = key_range<C::kTile>(p, len);
+            const int tiles = lane < p.batch ? r.tile_hi - r.tile_lo : 0;    // 32 of them: below 2^31
+            int upto = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
             }
+            total = static_cast<long long>(__shfl_sync(0xffffffffu, upto, 31)) * per_request;
+            const int shares = total < gridDim.x ? static_cast<int>(total) : static_cast<int>(gridDim.x);
+            if (share >= shares) return;             // fewer tiles than CTAs, so the cuts are told by unit
+            begin = share_begin(share, total, shares);
+            at = static_cast<long long>(upto - tiles) * per_request;
+            lb = __popc(__ballot_sync(0xffffffffu, lane < p.batch && at <= begin)) - 1;
+            len = __shfl_sync(0xffffffffu, len, lb);
+            at = __shfl_sync(0xffffffffu, at, lb);
+            to_load = static_cast<int>(share_begin(share + 1, total, shares) - begin);
+            if (tid == 0) s_total = total;           // (read again by this thread only)
+        } else {
+            const int chunk = (p.batch + kAttnThreads - 1) / kAttnThreads;
+            const int b_lo = min(tid * chunk, p.batch), b_hi = min(b_lo + chunk, p.batch);
+            long long mine = 0;
+            for (int b = b_lo; b < b_hi; ++b) {
+                const Range r = key_range<C::kTile>(p, p.lens[b]);
+                mine += static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
+            }
+            const long long upto = block_scan(mine, s_scan);
+            if (tid == kAttnThreads - 1) s_total = upto;
+            __syncthreads();
+            total = s_total;
+            const int shares = total < gridDim.x ? static_cast<int>(total) : static_cast<int>(gridDim.x);
+            if (share >= shares) return;
+            begin = share_begin(share, total, shares);
+            to_load = static_cast<int>(share_begin(share + 1, total, shares) - begin);
+            if (begin >= upto - mine && begin < upto) {
+                long long from = upto - mine;
+                for (int b = b_lo; b < b_hi; ++b) {
+                    const int length = p.lens[b];
+                    const Range r = key_range<C::kTile>(p, length);
+                    const long long n = static_cast<long long>(r.tile_hi - r.tile_lo) * per_request;
+                    if (begin < from + n) {
+                        s_request = b;
+                        s_len = length;
+                        s_at = from;
+                        break;
+                    }
+                    from += n;
+                }
+            }
+            __syncthreads();
+            lb = s_request;
+            len = s_len;
+            at = s_at;
         }
-        __syncthreads();
-        lb = s_request;
-        lr = key_range<C::kTile>(p, s_len);
-        const unsigned off = static_cast<unsigned>(begin - s_at);     // below tiles * per_request: 31 bits, checked
+        lr = key_range<C::kTile>(p, len);
+        const unsigned off = static_cast<unsigned>(begin - at);     // below tiles * per_request: 31 bits, checked
         const unsigned tiles = lr.tile_hi - lr.tile_lo;
         lu = off / tiles;
         lt = lr.tile_lo + off - lu * tiles;
@@ -789,6 +816,31 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     constexpr int RPI = 32 / CH;                     // rows that one instruction of the warp loads
     const bool one_page = p.page_size % KEYS == 0;   // a step's keys lie in one page
     const int lrow = lane / CH, lcol = (lane % CH) * 8;
+
+    // The query rows of a unit: to registers, or - where they go through shared memory - on their way to the L1.  Asked
+    // for ahead of the loads of keys, behind which they would wait: when the launch begins, and when a unit ends.
+    uint32_t qf[C::kQueryInSmem ? 1 : NT][C::kQueryInSmem ? 1 : KK][2];
+    auto ask_queries = [&](int b, int unit) {
+        const int hk = p.row_blocks == 1 ? unit : unit / p.row_blocks, row0 = (unit - hk * p.row_blocks) * ROWS;
+        const uint16_t* qrow = p.q + b * p.q_batch + (static_cast<long long>(hk) * p.group + row0) * p.q_head;
+        if constexpr (C::kQueryInSmem) {
+            constexpr int LINES = D / 64;
+            if (tid < ROWS * LINES && row0 + tid / LINES < p.group)
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(qrow + (tid / LINES) * p.q_head + (tid % LINES) * 64));
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int r = n * 8 + lane / 4;
+#pragma unroll
+                for (int k = 0; k < KK; ++k) {
+                    const uint16_t* x = qrow + r * p.q_head + k * 16 + (lane % 4) * 2;
+                    qf[n][k][0] = row0 + r < p.group ? *reinterpret_cast<const uint32_t*>(x) : 0u;
+                    qf[n][k][1] = row0 + r < p.group ? *reinterpret_cast<const uint32_t*>(x + 8) : 0u;
+                }
+            }
+        }
+    };
+    ask_queries(lb, lu);
 
     // The page of my key of the step at (lb, lt); looked up one step ahead, so that its latency is not waited for.
     // `found`: the key is visible; `row_in`: its row in the page.
@@ -812,7 +864,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         return;
     }
     float o[DT][NT][4], m[NT][2], l[NT][2];
-    uint32_t qf[C::kQueryInSmem ? 1 : NT][C::kQueryInSmem ? 1 : KK][2];
     bool fresh = true;               // a unit begins
     int stage = 0, ahead = STAGES - 1;               // steps to load before the first is waited for
     for (;;) {
@@ -886,8 +937,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         const int row0 = (st.unit - hk * p.row_blocks) * ROWS;               // first query head in the group
         if (fresh) {
             fresh = false;
-            const uint16_t* qrow = p.q + st.b * p.q_batch + (static_cast<long long>(hk) * p.group + row0) * p.q_head;
             if constexpr (C::kQueryInSmem) {
+                const uint16_t* qrow = p.q + st.b * p.q_batch + (static_cast<long long>(hk) * p.group + row0) * p.q_head;
                 // all four warps are here: the unit before has been joined, and the first begins with the launch
                 for (int i = tid; i < ROWS * CH; i += kAttnThreads) {
                     const int r = i / CH, c = i % CH;
@@ -895,17 +946,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
                     *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(join) + r * (D * 2) + ((c ^ (r & 7)) << 4)) = x;
                 }
                 __syncthreads();
-            } else {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int r = n * 8 + lane / 4;
-#pragma unroll
-                    for (int k = 0; k < KK; ++k) {
-                        const uint16_t* x = qrow + r * p.q_head + k * 16 + (lane % 4) * 2;
-                        qf[n][k][0] = row0 + r < p.group ? *reinterpret_cast<const uint32_t*>(x) : 0u;
-                        qf[n][k][1] = row0 + r < p.group ? *reinterpret_cast<const uint32_t*>(x + 8) : 0u;
-                    }
-                }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -1056,6 +1096,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
 
         // ---- the unit ends, or the share does: the four warps' results become one.  Each warp scales its own to the
         // maximum of the four; what is left is a sum, eight heads at a time through shared memory.
+        if (!C::kQueryInSmem && (st.last & 1) == 0) {
+            const Step& next = s_step[warp][stage];
+            ask_queries(next.b, next.unit);
+        }
         const bool whole = p.cluster <= 1 && from_begin && (st.last & 2) != 0;
         const int rows = min(p.group - row0, ROWS);
         const long long head0 = static_cast<long long>(st.b) * p.heads + hk * p.group + row0;

@@ -565,8 +565,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
 // Attention of one new token per request over the pages
 // ------------------------------------------------------------------------------------------------
 // Mathematics: one pass over the keys with a running reference m, a sum l and an accumulator o per query head, in
-// fp32 and in powers of two: x = log2(e) * score, p = 2^(x - m), l = sum p, o = sum p v.  m is a maximum that moves
-// only when a score exceeds it by more than 8 (p stays below 2^8, and o / l does not depend on m).  Parts of a
+// fp32 and in powers of two: x = log2(e) * score, p = 2^(x - m), l = sum p, o = sum p v.  m goes by a maximum that
+// moves only when a score exceeds it by more than 8 (o / l does not depend on m).  Parts of a
 // key range are joined by  o = sum_i 2^(m_i - m) o_i  and likewise l.
 //
 // Bound: memory.  A key of a KV head costs 4 * head_dim bytes and 4 * head_dim flops per query head of the
@@ -597,14 +597,19 @@ constexpr int kWarps = 4;
 constexpr int kAttnThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kGrowth = 8.f;         // how far (in powers of two) a score may exceed the reference m
+constexpr float kGrowth = 8.f;         // how far (in powers of two) a score may exceed the maximum that m goes by
+// m lies so far below that maximum.  Weights in fp16 vanish below 2^-25: with p up to 2^14 instead of 2^8, a hundred
+// thousand keys of such weights together stay below the rounding of the output.  (bf16 has fp32's exponents.)
+template <bool BF16>
+constexpr float kHeadroom = BF16 ? 0.f : 6.f;
 
 template <int D, int NT>
 struct AttnCfg {
     static constexpr int kKeys = 2048 / D;                 // keys of one warp's step: K and V are 4 KB each
     static constexpr int kTile = kKeys * kWarps;
     static constexpr int kStageBytes = kKeys * D * 2 * 2;
-    // Stages and CTAs per SM, by what fits 227 KB; measured beside the launch (launch_attention).
+    // Stages and CTAs per SM: what shared memory and registers allow.  24 to 32 KB in flight per warp and three stages
+    // read 6.4 of 6.5 TB/s; at 64, more warps hide the softmax, twice the work per byte (35 us against 77 with two CTAs).
     static constexpr int kStages = NT > 2 || D == 64 ? 2 : 3;
     static constexpr int kCtas = D == 64 && NT == 1 ? 3 : 2;
     static constexpr int kRingBytes = kStageBytes * kStages * kWarps;
@@ -1039,7 +1044,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
 #pragma unroll
                 for (int t = 1; t < MT; ++t) x = fmaxf(x, fmaxf(s[t][n][r], s[t][n][r + 2]));
                 top[n][r] = x;
-                grown |= x > m[n][r] + kGrowth;
+                grown |= x > m[n][r] + (kGrowth + kHeadroom<BF16>);
             }
         if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -1050,7 +1055,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    const float now = fmaxf(m[n][r], x);
+                    const float now = fmaxf(m[n][r], x - kHeadroom<BF16>);
                     const float f = exp2_approx(m[n][r] - finite_ref(now));
                     m[n][r] = now;
                     l[n][r] *= f;
@@ -1411,6 +1416,10 @@ struct AttnPlan {
     size_t cut_bytes, bytes;
 };
 
+static float score_inner(const FaPagedAttentionArgs* a) {
+    return a->softcap > 0.f ? static_cast<float>(2.0 * 1.4426950408889634 * a->scale / a->softcap) : 0.f;
+}
+
 static int check_attention(const FaPagedAttentionArgs* a) {
     if (a == nullptr) return FA_PAGED_ERR_NULL;
     if (a->struct_size != sizeof(FaPagedAttentionArgs)) return FA_PAGED_ERR_ABI;
@@ -1426,6 +1435,8 @@ static int check_attention(const FaPagedAttentionArgs* a) {
         static_cast<long long>(a->batch) * a->heads > INT_MAX)
         return FA_PAGED_ERR_SHAPE;
     if (a->window < 0 || !std::isfinite(a->scale) || !std::isfinite(a->softcap) || a->scale < 0.f || a->softcap < 0.f)
+        return FA_PAGED_ERR_SCORE;
+    if (!std::isfinite(a->scale * kLog2e) || !std::isfinite(a->softcap * kLog2e) || !std::isfinite(score_inner(a)))
         return FA_PAGED_ERR_SCORE;
     if (!aligned16(a->q) || !aligned16(a->out) || !stride8(a->q_batch_stride) || !stride8(a->q_head_stride))
         return FA_PAGED_ERR_ALIGN;
@@ -1526,8 +1537,9 @@ static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t byte
     p.q = static_cast<const uint16_t*>(a->q);
     p.out = static_cast<uint16_t*>(a->out);
     p.lse = a->lse;
-    p.k = static_cast<const uint16_t*>(c.k);
-    p.v = static_cast<const uint16_t*>(c.v);
+    // (a cache without pages: nothing is read, but what is copied as zeros names an address)
+    p.k = static_cast<const uint16_t*>(c.num_pages > 0 ? c.k : a->q);
+    p.v = static_cast<const uint16_t*>(c.num_pages > 0 ? c.v : a->q);
     p.table = a->block_table;
     p.lens = a->lens;
     p.slopes = a->slopes;
@@ -1540,7 +1552,7 @@ static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t byte
     const bool cap = a->softcap > 0.f;
     p.scale2 = a->scale * kLog2e;
     p.cap2 = a->softcap * kLog2e;
-    p.inner = cap ? static_cast<float>(2.0 * 1.4426950408889634 * a->scale / a->softcap) : 0.f;
+    p.inner = score_inner(a);
     int s = 0;
     while ((1LL << s) < c.page_size) ++s;
     p.page_mul = static_cast<unsigned>(((1ULL << (31 + s)) + c.page_size - 1) / c.page_size);

@@ -12,7 +12,7 @@
  * FA_PAGED_ERR_* code, never throws, never synchronises, never allocates; memory belongs to the caller;
  * work is enqueued on the caller's stream, chained to the kernel before it (every kernel waits for that
  * one before it touches memory).  No kernel here waits for another one's memory, so there is no status
- * word.  Pointers are device pointers on `device`; `struct_size` is sizeof of the struct, checked.
+ * word.  The first call of an operator on a device loads its kernel: make it outside any stream capture.  Pointers are device pointers on `device`; `struct_size` is sizeof of the struct, checked.
  *
  * The cache: pages of `page_size` tokens, k and v each (num_pages, heads_k, page_size, head_dim) of one
  * 16-bit type, addressed through their element strides (page, head, token); the last dimension is
@@ -77,7 +77,7 @@ typedef struct FaPagedCache {
  *   slots[t]         for t < num_tokens: the token's slot; -1 for a token of a refused request and
  *                    behind the last one (padding)
  *   positions[t]     lens[b] + its index among the request's new tokens; 0 behind the last one
- * lens_out may be lens and head_out may be free_head (updated in place).  Requests are extended in full
+ * The sum of new_lens must be below 2^31.  lens_out may be lens and head_out may be free_head (updated in place).  Requests are extended in full
  * also where num_tokens is smaller than cu[batch].
  */
 typedef struct FaPagedExtendArgs {

@@ -164,6 +164,49 @@ def test_attention_of_few_short_requests(d, H, Hk):
             attend_and_check(*args, what=f"{columns} columns, {B} requests", window=tile + 3)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_of_many_small_weights(dtype):
+    """One key takes most; each of 60000 others has a weight of 2^-25.4 of it, below fp16's smallest number, and
+    together they are three roundings of the output."""
+    n, d = 60001, 64
+    q, k, v, table, lens = make_cache([n], H=4, Hk=1, d=d, page_size=16, dtype=dtype, gen=gen(9))
+    q.zero_()
+    q[..., 0] = 1.0
+    k.zero_()
+    key = 12345
+    k[table[0, key // 16].long(), :, key % 16, 0] = 17.6 if dtype == torch.float16 else 17.625
+    v.abs_()
+    attend_and_check(q, k, v, table, lens, scale=1.0)
+
+
+def test_attention_over_a_cache_without_pages():
+    q, k, v, table, lens = make_cache([30, 0], H=4, Hk=2, d=128, page_size=16, dtype=torch.float16, gen=gen(1))
+    out, lse = ops.paged_attention_lse(q, k[:0], v[:0], table, lens)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_operators_through_compile():
+    """As the framework's other operators: traced by their fake kernels, mutations of the caches included."""
+    q, k, v, table, lens = make_cache([30, 1, 99], H=4, Hk=2, d=64, page_size=16, dtype=torch.bfloat16, gen=gen(3))
+    freqs, _ = rotary_frequencies(64, 10000.0)
+    new = torch.randn(3, 8, 64, device="cuda").bfloat16()
+
+    def step(q, new, kc, vc, table, lens, free, head):
+        one = torch.ones_like(lens)
+        lens, head, slots, positions, _ = ops.paged_extend(table, lens, one, free, head, 16, 3)
+        q = ops.rotary_append(new[:, :4], new[:, 4:6], new[:, 6:], positions, slots, kc, vc, freqs)
+        return ops.paged_attention(q, kc, vc, table, lens, softcap=20.0), lens, slots
+
+    ops.ensure_loaded("paged")
+    got = []
+    for f in (step, torch.compile(step, backend="aot_eager", fullgraph=True)):
+        state = [x.clone() for x in (k, v, table, lens)]
+        free, head = torch.tensor([k.shape[0] - 1, k.shape[0] - 2], dtype=torch.int32, device="cuda"), torch.zeros_like(lens[:1])
+        got.append([*f(q, new, *state, free, head), *state])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_attention_passes_nan_on():
     """A NaN that a row may see is its result, in every way of dividing the work up; other rows are untouched."""
     for length in (40, 700, 9000):

@@ -79,7 +79,7 @@ def attention(**kw):
     (dict(cache__k=P + 8), -5), (dict(q=P + 2), -5), (dict(out=P + 4), -5), (dict(q_head_stride=68), -5),
     (dict(cache__v_row_stride=65), -5), (dict(cache__k_page_stride=-8), -5),
     (dict(window=-1), -10), (dict(softcap=-1.0), -10), (dict(softcap=float("nan")), -10), (dict(scale=float("inf")), -10),
-    (dict(scale=-0.5), -10), (dict(table_width=1 << 28), -3), (dict(batch=1 << 20, heads=1 << 12), -3),
+    (dict(scale=-0.5), -10), (dict(scale=3e38), -10), (dict(softcap=1e-45), -10), (dict(table_width=1 << 28), -3), (dict(batch=1 << 20, heads=1 << 12), -3),
 ])
 def test_attention_refusals(kw, code):
     with pytest.raises(abi.PagedError) as e:

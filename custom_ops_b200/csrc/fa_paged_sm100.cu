@@ -181,7 +181,7 @@ __device__ __forceinline__ void block_scan2(long long& a, long long& b, long lon
 // 48 prompts, 79,000 tokens and 5,000 pages: 12.4 us a call, 77 with one CTA and a token at a time.
 constexpr int kTableThreads = 512, kTableClusterThreads = 1024;      // of the one CTA, of each of the eight
 constexpr int kTableCluster = 8;
-constexpr long long kTableTokens = 4096;
+constexpr long long kTableTokens = 4096;       // both the host's 10 us up to 8,000 tokens; 16,000: 12.2 us against 16.5
 
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
@@ -407,6 +407,7 @@ constexpr int kRotaryThreads = 128;
 constexpr int kRotaryBatch = 3;
 constexpr int kRotaryTokens = 8;
 constexpr int kRotaryWaves = 4;       // CTAs per SM that there have to be
+// (One token a CTA: 21.7 us instead of 15.7 for 20 heads of 128, 19.4 instead of 11.9 for 8100 tokens with 12.)
 
 struct Rows {                     // heads of one token: where they are read and where they go
     const uint16_t* in;
@@ -757,7 +758,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         lb = unit / per_request;
         lu = unit - lb * per_request;
         lr = key_range<C::kTile>(p, p.lens[lb]);
-        const int tiles = lr.tile_hi - lr.tile_lo;       // 8 CTAs at most, of kUnitTiles tiles
+        const int tiles = lr.tile_hi - lr.tile_lo;       // 8 CTAs at most, of ten tiles
         lt = lr.tile_lo + tiles * rank / p.cluster;
         to_load = lr.tile_lo + tiles * (rank + 1) / p.cluster - lt;
     } else {
@@ -834,7 +835,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
 
     constexpr int CH = D / 8;                        // 16-byte chunks of a row
     constexpr int RPI = 32 / CH;                     // rows that one instruction of the warp loads
-    const bool one_page = p.page_size % KEYS == 0;   // a step's keys lie in one page
     const int lrow = lane / CH, lcol = (lane % CH) * 8;
 
     // The query rows of a unit: to registers, or - where they go through shared memory - on their way to the L1.  Asked
@@ -896,35 +896,16 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
             const uint16_t* vb = p.v + hk * p.v_head + lcol;
             const int load_stage = ahead > 0 ? STAGES - 1 - ahead : stage == 0 ? STAGES - 1 : stage - 1;
             const uint32_t dst = ring_u + load_stage * C::kStageBytes;
-            if (one_page) {
-                // the first key that can be seen names the page; rows ahead of it and behind the last are not read
-                const int from = mask != 0 ? __ffs(mask) - 1 : 0;
-                const long long pg = mask != 0 ? __shfl_sync(0xffffffffu, page, from) : 0;
-                const int r0 = __shfl_sync(0xffffffffu, row_in, from) - from + lrow;
-                kb += pg * p.k_page + r0 * p.k_row;
-                vb += pg * p.v_page + r0 * p.v_row;
-#pragma unroll
-                for (int i = 0; i < KEYS / RPI; ++i) {
-                    const int row = i * RPI + lrow;
-                    const uint32_t bytes = (mask >> row) & 1u ? 16u : 0u;
-                    const uint32_t at = dst + row * (D * 2) + (((lane % CH) ^ (row & 7)) << 4);
-                    cp_async16(at, bytes ? kb : p.k, bytes);
-                    cp_async16(at + KEYS * D * 2, bytes ? vb : p.v, bytes);
-                    kb += RPI * p.k_row;
-                    vb += RPI * p.v_row;
-                }
-            } else {
-                const bool ok = (mask >> (lane % KEYS)) & 1u;
-                const long long ko = ok ? page * p.k_page + row_in * p.k_row : 0, vo = ok ? page * p.v_page + row_in * p.v_row : 0;
-#pragma unroll 2
-                for (int i = 0; i < KEYS / RPI; ++i) {
-                    const int row = i * RPI + lrow;
-                    const long long kro = __shfl_sync(0xffffffffu, ko, row), vro = __shfl_sync(0xffffffffu, vo, row);
-                    const uint32_t bytes = (mask >> row) & 1u ? 16u : 0u;
-                    const uint32_t at = dst + row * (D * 2) + (((lane % CH) ^ (row & 7)) << 4);
-                    cp_async16(at, kb + kro, bytes);
-                    cp_async16(at + KEYS * D * 2, vb + vro, bytes);
-                }
+            const bool ok = (mask >> (lane % KEYS)) & 1u;
+            const long long ko = ok ? page * p.k_page + row_in * p.k_row : 0, vo = ok ? page * p.v_page + row_in * p.v_row : 0;
+#pragma unroll(NT > 2 ? 4 : KEYS / RPI)
+            for (int i = 0; i < KEYS / RPI; ++i) {
+                const int row = i * RPI + lrow;
+                const long long kro = __shfl_sync(0xffffffffu, ko, row), vro = __shfl_sync(0xffffffffu, vo, row);
+                const uint32_t bytes = (mask >> row) & 1u ? 16u : 0u;
+                const uint32_t at = dst + row * (D * 2) + (((lane % CH) ^ (row & 7)) << 4);
+                cp_async16(at, kb + kro, bytes);
+                cp_async16(at + KEYS * D * 2, vb + vro, bytes);
             }
             if (lane == 0) {
                 Step& st = s_step[warp][load_stage];
@@ -1419,9 +1400,12 @@ static int launch_rotary(const RotaryParams& p, bool interleaved, long long toke
 }
 
 // Short units: each is done by a cluster of 1 to 8 CTAs that join their parts through their shared memory.  No sums
-// over the lengths, no partial results in memory, no second kernel (which costs the host 2 us, too).  Up to so many
-// tiles for a CTA, as long as the CTAs all run at once; with more, equal shares of all keys pay for what they take.
-constexpr int kUnitTiles = 8;
+// over the lengths, no partial results in memory, no second kernel (which costs the host 2.7 us, too).  Up to so many
+// tiles for a CTA: 4, and 6 more as the clusters fill the GPU, where equal shares of all keys have no SMs to win.  GPU
+// time with clusters and with equal shares, 4 KV heads of 128: one request of 300 keys 5.9 and 6.5 us, of 2000 (4 tiles
+// a CTA) 7.9 and 6.9, of 3000 9.7 and 7.2; 4 requests of 2500 (5) 9.1 and 9.3, of 4000 12.0 and 10.0; 8 of 4000 (8) 15.0
+// and 15.5; 16 of 2000 (8) 14.8 and 16.1, of 3000 (12) 19.4 and 19.0.
+constexpr int kUnitTiles = 4, kUnitTilesFull = 6;
 constexpr int kMostCluster = 8;
 
 struct AttnPlan {
@@ -1462,6 +1446,9 @@ static int check_attention(const FaPagedAttentionArgs* a) {
 template <int D>
 static int make_attn_plan(const FaPagedAttentionArgs* a, int sms, AttnPlan* plan) {
     const int group = a->heads / a->cache.heads_k;
+    // Query heads of a tile: as many as the group has.  16 requests of 16384 keys on one key head: 8 heads 23.9 us (with
+    // tiles of 16: 25.1), 12 heads 26.1 (of 8, twice: 32.5; of 32: 30.8), 16 heads 27.1 (32.9; 31.2), 32 heads 37.1 (of 16,
+    // twice: 41.0).
     plan->nt = group <= 8 ? 1 : group <= 16 ? 2 : 4;
     plan->row_blocks = (group + plan->nt * 8 - 1) / (plan->nt * 8);
     const long long capacity = static_cast<long long>(a->table_width) * a->cache.page_size;
@@ -1475,9 +1462,10 @@ static int make_attn_plan(const FaPagedAttentionArgs* a, int sms, AttnPlan* plan
     const long long seen = a->window > 0 && a->window < capacity ? a->window / attn_tile(D) + 2 : tiles;      // of one unit, at most
     int cluster = 1;
     while (cluster < kMostCluster && 2 * cluster <= seen && 2 * cluster * units <= resident) cluster *= 2;
-    if (seen <= 1 || (seen <= static_cast<long long>(kUnitTiles) * cluster && units * cluster <= resident)) {
+    const long long ctas = units * cluster;
+    if (seen <= 1 || (ctas <= resident && seen <= cluster * (kUnitTiles + kUnitTilesFull * ctas / resident))) {
         plan->cluster = cluster;
-        plan->grid = static_cast<int>(units * cluster);
+        plan->grid = static_cast<int>(ctas);
         return FA_PAGED_OK;
     }
     plan->grid = static_cast<int>(most < resident ? most : resident);

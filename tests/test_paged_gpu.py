@@ -140,7 +140,9 @@ def test_attention_offsets_beyond_32_bits():
 
 
 @pytest.mark.parametrize("B,H,Hk,d,length", [(1, 8, 1, 128, 70001), (1, 32, 8, 128, 20000), (2, 4, 4, 64, 33333),
-                                             (37, 8, 4, 128, 900), (300, 4, 2, 64, 65), (1500, 2, 1, 64, 20)])
+                                             (37, 8, 4, 128, 900), (300, 4, 2, 64, 65), (1500, 2, 1, 64, 20),
+                                             (200, 8, 4, 128, 700), (160, 6, 3, 64, 2500), (60, 40, 5, 128, 1200),
+                                             (40, 32, 1, 128, 5000), (33, 12, 1, 64, 4000)])
 def test_attention_split_over_the_gpu(B, H, Hk, d, length):
     """Long and many: shares begin and end anywhere.  The same call gives the same bits."""
     r = random.Random(B)
@@ -149,6 +151,16 @@ def test_attention_split_over_the_gpu(B, H, Hk, d, length):
     got = attend_and_check(*args)
     for _ in range(3):
         assert torch.equal(ops.paged_attention(*args), got)
+
+
+@pytest.mark.parametrize("d,H,Hk", [(128, 8, 2), (64, 4, 4), (128, 32, 1)])
+def test_attention_of_one_long_among_many_short(d, H, Hk):
+    """Shares that hold hundreds of ends of units, and a unit that is cut in most of the parts."""
+    for B in (5, 31, 32, 33, 150, 700):
+        lens = [(0, 1, 70)[b % 3] for b in range(B)]
+        lens[B // 2] = 30000
+        args = make_cache(lens, H=H, Hk=Hk, d=d, page_size=64, dtype=torch.bfloat16, gen=gen(B))
+        attend_and_check(*args, what=f"{B} requests")
 
 
 @pytest.mark.parametrize("d,H,Hk", [(128, 8, 2), (64, 3, 3), (128, 32, 1), (64, 24, 2)])

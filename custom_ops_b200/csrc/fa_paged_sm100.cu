@@ -28,8 +28,8 @@ namespace fa_paged {
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-// Lets the next kernel of the stream become resident / waits until the kernel before has finished.  The attention
-// kernels do not announce the next one early: resident CTAs of the next take their places SM by SM as theirs
+// Lets the next kernel of the stream become resident / waits until the kernel before has finished.  The rotary
+// and attention kernels do not announce the next one early: resident CTAs of the next take their places SM by SM as theirs
 // leave, which spread the next call unevenly (48 requests, 16 heads of 64: 53 us a call with it, 40 without).
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

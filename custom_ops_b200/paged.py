@@ -11,7 +11,7 @@ positions.  The reference has no counterpart.
         out = cache.attend(layer, q)                                   # a step of one token per request
     cache.release(rows)                                                # pages of finished requests
 
-Nothing here synchronises: a step may be captured into a CUDA graph and replayed.
+Nothing here synchronises: after one step outside a capture, a step may be captured into a CUDA graph and replayed.
 """
 from __future__ import annotations
 
@@ -123,7 +123,8 @@ class PagedCache:
         ops.paged_shrink_(self.block_table, self.seq_lens, keep_lens, self.free_pages, self.free_head, self.page_size)
 
     def release(self, rows: torch.Tensor) -> None:
-        """Frees all pages of the requests in ``rows`` (an index or boolean tensor, or a list)."""
+        """Frees all pages of the requests in ``rows``: an index or boolean tensor on the device, or a list (which is
+        copied there)."""
         keep = self.seq_lens.clone()
         keep[rows] = 0
         self.shrink(keep)

@@ -134,8 +134,12 @@ def test_attention_offsets_beyond_32_bits():
     want = ops.paged_attention(q, small, small, torch.arange(5, dtype=torch.int32, device="cuda").view(1, 5), lens)
     assert torch.equal(ops.paged_attention(q, k, k, table, lens), want)
     by_head = k.view(Hk, P, ps, d).transpose(0, 1)
+    rows = small.transpose(1, 2).reshape(-1, Hk, d)                      # written by the append, token by token
+    slots = torch.cat([torch.arange(p * ps, (p + 1) * ps) for p in pages]).cuda()
+    by_head_v = torch.empty_like(k).view(Hk, P, ps, d).transpose(0, 1)
+    ops.paged_append(rows, rows, slots, by_head, by_head_v)
     for p in pages:
-        by_head[p] = small[pages.index(p)]
+        assert torch.equal(by_head[p], small[pages.index(p)]) and torch.equal(by_head_v[p], by_head[p])
     assert torch.equal(ops.paged_attention(q, by_head, by_head, table, lens), want)
 
 
@@ -489,6 +493,17 @@ def test_rotary_shapes_and_refusals():
             ops.rotary(*args)
     with pytest.raises(RuntimeError):
         ops.rotary(x, x, p, freqs, mscale=float("nan"))
+
+
+def test_rotary_offsets_beyond_32_bits():
+    """More than 2^31 elements in and out, rows one behind the other and interleaved by head."""
+    H, S, d = 33, 2 ** 19 + 3, 128
+    q = torch.empty(1, S, H, d, dtype=torch.float16, device="cuda").transpose(1, 2)
+    at = torch.tensor([0, 1, S // 2, S - 2, S - 1], device="cuda")
+    q[:, :, at] = torch.randn(1, H, 5, d, device="cuda").half()
+    freqs, _ = rotary_frequencies(d, 10000.0)
+    out, _ = ops.rotary(q, q[:, :0], torch.arange(S, device="cuda"), freqs)
+    check_turned(out[:, :, at], turn_reference(q[:, :, at], at, freqs))
 
 
 # ------------------------------------------------------------------ append

@@ -121,6 +121,26 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
     else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
+// The page size, as a divisor of numbers below 2^31:  x / size = x * mul >> shift,  shift = 31 + ceil(log2(size)),
+// mul = ceil(2^shift / size).  (mul is off by less than 1, so the product is by less than x < 2^31, a quotient by less
+// than 1 / size.)
+struct PageSize {
+    unsigned size, mul, shift;
+};
+static PageSize page_size_of(int size) {
+    unsigned s = 31;
+    while ((1ULL << (s - 31)) < static_cast<unsigned long long>(size)) ++s;
+    return PageSize{static_cast<unsigned>(size), static_cast<unsigned>(((1ULL << s) + size - 1) / size), s};
+}
+__device__ __forceinline__ unsigned page_of(unsigned token, const PageSize& ps) {
+    return static_cast<unsigned>((static_cast<unsigned long long>(token) * ps.mul) >> ps.shift);
+}
+// Pages of so many tokens.
+__device__ __forceinline__ unsigned pages_of(unsigned tokens, const PageSize& ps) {
+    const unsigned whole = page_of(tokens, ps);
+    return whole + (whole * ps.size != tokens);
+}
+
 __device__ __forceinline__ long long load_int(const void* p, int is64, long long i) {
     return is64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
 }
@@ -177,10 +197,12 @@ __device__ __forceinline__ void block_scan2(long long& a, long long& b, long lon
 // reads (lengths, free list, table).  Small calls are one CTA; from kTableTokens on it is a cluster of eight, each
 // of which works out the (cheap) sums for itself and takes an eighth of the tokens and pages.  A cluster and not
 // a grid, because lens and free_head may be updated in place: they are written behind a cluster barrier, when
-// every CTA has read them.  256 decoding requests: 10 us a call, the host's time (the kernel with cold caches: 10.4);
-// 48 prompts, 79,000 tokens and 5,000 pages: 12.4 us a call, 77 with one CTA and a token at a time.
+// every CTA has read them.  Replayed from a graph: 256 decoding requests 3.5 us (8.0 with a warp per request for its
+// pages, four tokens a thread and divisions); 48 prompts, 79,000 tokens and 5,000 pages: 10.5 us; called from Python both
+// take the host's 10 us.  With one CTA the prompts took 70 us.
 constexpr int kTableThreads = 512, kTableClusterThreads = 1024;      // of the one CTA, of each of the eight
 constexpr int kTableCluster = 8;
+constexpr int kFewPages = 4;           // that the thread of a request hands out by itself
 constexpr long long kTableTokens = 4096;       // both the host's 10 us up to 8,000 tokens; 16,000: 12.2 us against 16.5
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -208,14 +230,11 @@ struct ExtendParams {
     long long* slots;
     int* positions;
     int* cu;
-    int batch, width, page_size, num_free;
+    PageSize page;
+    int batch, width, num_free;
     long long num_tokens;
 };
 
-// Pages of so many tokens; no overflow, whatever is in the lengths.
-__device__ __forceinline__ unsigned pages_of(unsigned tokens, unsigned page_size) {
-    return tokens / page_size + (tokens % page_size != 0);
-}
 
 __global__ void __launch_bounds__(kTableClusterThreads) paged_extend_kernel(const ExtendParams p) {
     extern __shared__ int s_table[];
@@ -237,12 +256,16 @@ __global__ void __launch_bounds__(kTableClusterThreads) paged_extend_kernel(cons
         s_before[0] = s_before[1] = 0;
     }
     __syncthreads();
+    bool many = false;                      // some request gets more than a few pages
     for (int base = 0; base < p.batch; base += threads) {
         const int b = base + tid;
         const bool in = b < p.batch;
         const unsigned len = in ? max(p.lens[b], 0) : 0, add = in ? max(p.new_lens[b], 0) : 0;
-        const unsigned have = pages_of(len, p.page_size), want = pages_of(len + add, p.page_size);
-        const bool fits = want <= static_cast<unsigned>(p.width);
+        const unsigned have = pages_of(len, p.page);
+        unsigned want = have;
+        const bool counted = len + add <= static_cast<unsigned>(INT_MAX);
+        if (counted) want = pages_of(len + add, p.page);
+        const bool fits = counted && want <= static_cast<unsigned>(p.width);
         const unsigned need = fits ? want - have : 0;
         long long tokens = add, pages = need;
         block_scan2(tokens, pages, s_scan);
@@ -252,8 +275,15 @@ __global__ void __launch_bounds__(kTableClusterThreads) paged_extend_kernel(cons
         if (in) {
             s_cu[b + 1] = static_cast<int>(min(tokens, static_cast<long long>(INT_MAX)));
             s_len[b] = static_cast<int>(len);
-            s_src[b] = !granted ? -1 : need > 0 ? head + static_cast<int>(pages) - static_cast<int>(need) : 0;
+            const int src = head + static_cast<int>(pages) - static_cast<int>(need);
+            s_src[b] = !granted ? -1 : need > 0 ? src : 0;
+            // a few pages: here and now
+            if (granted && need > 0 && need <= kFewPages && b % ranks == rank) {
+                int* row = p.table + b * p.table_stride + have;
+                for (unsigned i = 0; i < need; ++i) row[i] = p.free_pages[src + i];
+            }
         }
+        many |= in && granted && need > kFewPages;
         // pages are given to a first part of those that need some: the last prefix sum there is their number
         const int given = __reduce_max_sync(0xffffffffu, in && granted && need > 0 ? head + static_cast<int>(pages) : 0);
         if ((tid & 31) == 0 && given > 0) atomicMax(&s_head, given);
@@ -265,21 +295,24 @@ __global__ void __launch_bounds__(kTableClusterThreads) paged_extend_kernel(cons
         __syncthreads();
     }
     cluster_arrive();                       // lens and free_head have been read
-    const unsigned page_size = p.page_size;
-    // new pages: one warp per request
-    const int warps = ranks * (threads / 32);
-    for (int b = rank * (threads / 32) + (tid >> 5); b < p.batch; b += warps) {
-        if (s_src[b] < 0) continue;
-        const unsigned len = s_len[b], add = s_cu[b + 1] - s_cu[b];      // len + add: countable in 31 bits, or refused
-        const int have = pages_of(len, page_size), want = pages_of(len + add, page_size);
-        int* row = p.table + b * p.table_stride;
-        for (int i = have + (tid & 31); i < want; i += 32) row[i] = p.free_pages[s_src[b] + i - have];
+    if (__syncthreads_or(many)) {
+        // many pages: one warp per request
+        const int warps = ranks * (threads / 32);
+        for (int b = rank * (threads / 32) + (tid >> 5); b < p.batch; b += warps) {
+            if (s_src[b] < 0) continue;
+            const unsigned len = s_len[b], add = s_cu[b + 1] - s_cu[b];
+            const int have = pages_of(len, p.page), want = pages_of(len + add, p.page);
+            if (want - have <= kFewPages) continue;
+            int* row = p.table + b * p.table_stride;
+            for (int i = have + (tid & 31); i < want; i += 32) row[i] = p.free_pages[s_src[b] + i - have];
+        }
     }
     // slots and positions; a page that is new is read from the free list, not from the row just written
     const long long total = s_cu[p.batch];
     const bool vec = ((reinterpret_cast<uintptr_t>(p.slots) | reinterpret_cast<uintptr_t>(p.positions)) & 15u) == 0;
-    for (long long t0 = 4 * (static_cast<long long>(rank) * threads + tid); t0 < p.num_tokens;
-         t0 += 4LL * ranks * threads) {
+    const int each = p.num_tokens <= static_cast<long long>(ranks) * threads ? 1 : 4;     // tokens that a thread takes at a time
+    for (long long t0 = each * (static_cast<long long>(rank) * threads + tid); t0 < p.num_tokens;
+         t0 += static_cast<long long>(each) * ranks * threads) {
         const int* from[4];                              // where the page of each token is named
         unsigned row[4];
         int pos[4];
@@ -296,13 +329,13 @@ __global__ void __launch_bounds__(kTableClusterThreads) paged_extend_kernel(cons
             from[e] = nullptr;
             row[e] = 0;
             pos[e] = 0;
-            if (t < total) {
+            if (e < each && t < total) {
                 while (s_cu[b + 1] <= t) ++b;
                 pos[e] = static_cast<int>(s_len[b] + (t - s_cu[b]));
                 if (s_src[b] >= 0) {
-                    const unsigned have = pages_of(s_len[b], page_size), at = static_cast<unsigned>(pos[e]) / page_size;
+                    const unsigned have = pages_of(s_len[b], p.page), at = page_of(pos[e], p.page);
                     from[e] = at < have ? p.table + b * p.table_stride + at : p.free_pages + s_src[b] + (at - have);
-                    row[e] = static_cast<unsigned>(pos[e]) - at * page_size;
+                    row[e] = static_cast<unsigned>(pos[e]) - at * p.page.size;
                 }
             }
         }
@@ -311,15 +344,15 @@ __global__ void __launch_bounds__(kTableClusterThreads) paged_extend_kernel(cons
 #pragma unroll
         for (int e = 0; e < 4; ++e) page[e] = from[e] != nullptr ? *from[e] : 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) slot[e] = from[e] != nullptr ? static_cast<long long>(page[e]) * page_size + row[e] : -1;
-        if (vec && t0 + 4 <= p.num_tokens) {
+        for (int e = 0; e < 4; ++e) slot[e] = from[e] != nullptr ? static_cast<long long>(page[e]) * p.page.size + row[e] : -1;
+        if (vec && each == 4 && t0 + 4 <= p.num_tokens) {
             *reinterpret_cast<longlong2*>(p.slots + t0) = make_longlong2(slot[0], slot[1]);
             *reinterpret_cast<longlong2*>(p.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
             *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (t0 + e < p.num_tokens) {
+                if (e < each && t0 + e < p.num_tokens) {
                     p.slots[t0 + e] = slot[e];
                     p.positions[t0 + e] = pos[e];
                 }
@@ -343,7 +376,8 @@ struct ShrinkParams {
     const int* keep;
     int* free_pages;
     int* free_head;
-    int batch, width, page_size, num_free;
+    PageSize page;
+    int batch, width, num_free;
 };
 
 __global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const ShrinkParams p) {
@@ -369,7 +403,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const Shrin
         const unsigned len = in ? max(p.lens[b], 0) : 0;
         const unsigned keep = in ? min(static_cast<unsigned>(max(p.keep[b], 0)), len) : 0;
         const unsigned most = p.width;
-        const unsigned from = min(pages_of(keep, p.page_size), most), upto = min(pages_of(len, p.page_size), most);
+        const unsigned from = min(pages_of(keep, p.page), most), upto = min(pages_of(len, p.page), most);
         const unsigned count = upto - from;
         const long long sum = s_before + block_scan(count, s_scan);
         const bool granted = count == 0 || sum <= head;
@@ -654,9 +688,9 @@ struct AttnParams {
     const float* slopes;
     long long q_batch, q_head, table_stride;
     long long k_page, k_head, k_row, v_page, v_head, v_row;
-    int batch, heads, heads_k, group, row_blocks, width, page_size, num_pages, window;
+    int batch, heads, heads_k, group, row_blocks, width, num_pages, window;
     int cluster;                  // n > 0: unit u is done by the n CTAs from n u on, a cluster; 0: equal shares
-    unsigned page_mul, page_shift;      // key / page_size = key * page_mul >> page_shift, for keys below 2^31
+    PageSize page;
     // x, in powers of two, is s * scale2, or with a cap  cap2 * tanh(s * inner / 2),  inner = 2 log2(e) scale / cap:
     // tanh(y) = 1 - 2 / (1 + 2^(2 log2(e) y))
     float scale2, cap2, inner;
@@ -678,7 +712,7 @@ struct Range {
 };
 template <int TILE>
 __device__ __forceinline__ Range key_range(const AttnParams& p, int len) {
-    const int most = p.width * p.page_size;
+    const int most = p.width * static_cast<int>(p.page.size);
     Range r;
     r.hi = min(max(len, 0), most);
     r.lo = p.window > 0 ? max(0, r.hi - p.window) : 0;
@@ -891,9 +925,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         const int key = lt * C::kTile + warp * KEYS + (lane % KEYS);
         found = key >= lr.lo && key < lr.hi;
         if (found) {
-            const int at = static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(key)) * p.page_mul) >> p.page_shift);
+            const int at = page_of(key, p.page);
             page = p.table[lb * p.table_stride + at];
-            row_in = key - at * p.page_size;
+            row_in = key - at * static_cast<int>(p.page.size);
         }
     };
     look_up();
@@ -1573,16 +1607,12 @@ static int attention(const FaPagedAttentionArgs* a, void* workspace, size_t byte
     p.k_page = c.k_page_stride, p.k_head = c.k_head_stride, p.k_row = c.k_row_stride;
     p.v_page = c.v_page_stride, p.v_head = c.v_head_stride, p.v_row = c.v_row_stride;
     p.batch = a->batch, p.heads = a->heads, p.heads_k = c.heads_k, p.group = a->heads / c.heads_k;
-    p.row_blocks = plan.row_blocks, p.width = a->table_width, p.page_size = c.page_size, p.num_pages = c.num_pages;
+    p.row_blocks = plan.row_blocks, p.width = a->table_width, p.page = page_size_of(c.page_size), p.num_pages = c.num_pages;
     p.window = a->window;
     const bool cap = a->softcap > 0.f;
     p.scale2 = a->scale * kLog2e;
     p.cap2 = a->softcap * kLog2e;
     p.inner = score_inner(a);
-    int s = 0;
-    while ((1LL << s) < c.page_size) ++s;
-    p.page_mul = static_cast<unsigned>(((1ULL << (31 + s)) + c.page_size - 1) / c.page_size);
-    p.page_shift = 31 + s;
     p.cluster = plan.cluster;
     p.cuts = static_cast<CutInfo*>(workspace);
     p.cuts_by_unit = plan.cuts < plan.grid;
@@ -1712,7 +1742,7 @@ static int extend(const FaPagedExtendArgs* a, cudaStream_t stream) {
     p.table = a->block_table, p.table_stride = a->table_stride, p.lens = a->lens, p.new_lens = a->new_lens;
     p.free_pages = a->free_pages, p.free_head = a->free_head, p.lens_out = a->lens_out, p.head_out = a->head_out;
     p.slots = reinterpret_cast<long long*>(a->slots), p.positions = a->positions, p.cu = a->cu;
-    p.batch = a->batch, p.width = a->table_width, p.page_size = a->page_size, p.num_free = a->num_free_pages;
+    p.batch = a->batch, p.width = a->table_width, p.page = page_size_of(a->page_size), p.num_free = a->num_free_pages;
     p.num_tokens = a->num_tokens;
     const int ctas = a->num_tokens >= kTableTokens ? kTableCluster : 1;
     return launch_cluster(paged_extend_kernel, dim3(ctas), ctas > 1 ? kTableClusterThreads : kTableThreads, (3 * static_cast<size_t>(a->batch) + 1) * 4, ctas,
@@ -1734,7 +1764,7 @@ static int shrink(const FaPagedShrinkArgs* a, cudaStream_t stream) {
     ShrinkParams p = {};
     p.table = a->block_table, p.table_stride = a->table_stride, p.lens = a->lens, p.keep = a->keep_lens;
     p.free_pages = a->free_pages, p.free_head = a->free_head;
-    p.batch = a->batch, p.width = a->table_width, p.page_size = a->page_size, p.num_free = a->num_free_pages;
+    p.batch = a->batch, p.width = a->table_width, p.page = page_size_of(a->page_size), p.num_free = a->num_free_pages;
     return launch_chained(paged_shrink_kernel, dim3(1), kTableThreads, 3 * static_cast<size_t>(a->batch) * 4, stream, p);
 }
 

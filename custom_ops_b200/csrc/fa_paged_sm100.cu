@@ -774,7 +774,9 @@ __device__ __forceinline__ void join_cluster(const AttnParams& p, const float* p
     cluster_wait();                  // and have been read
 }
 
-template <int D, bool BF16, int NT, bool CAP>
+// ALONE: every warp takes whole units, every so-manieth, by itself - for many short ones.  Else the four warps of a CTA
+// take the keys of a tile together.
+template <int D, bool BF16, int NT, bool CAP, bool ALONE>
 __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_attention_kernel(const AttnParams p) {
     using C = AttnCfg<D, NT>;
     constexpr int MT = C::kKeys / 16, KK = D / 16, DT = D / 16, KEYS = C::kKeys, STAGES = C::kStages;
@@ -790,13 +792,28 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     const int per_request = p.heads_k * p.row_blocks, share = blockIdx.x;
 
     // ---- my share; the loader's place: request, unit within the request, tile
-    int lb, lu, lt, left;                            // left: places of the share still to be loaded
+    constexpr int TILE = ALONE ? KEYS : C::kTile;    // keys of a place in the sequence
+    int lb, lu, lt, left;                            // left: places of the share (ALONE: of the unit) still to be loaded
     int gap = 0;                                     // places that the end of a unit counts as
     Range lr;
-    if (p.cluster > 0) {
-        const int rank = static_cast<int>(cluster_rank()), unit = share / p.cluster;
+    // ALONE: the unit that is loaded, the step to the next, all of them, and the next one's length, asked for ahead
+    int unit = share * kWarps + warp, next_len = 0;
+    const int stride = static_cast<int>(gridDim.x) * kWarps, units = p.batch * per_request;
+    auto begin_unit = [&](int len) {
         lb = unit / per_request;
         lu = unit - lb * per_request;
+        lr = key_range<TILE>(p, len);
+        lt = lr.tile_lo;
+        left = lr.tile_hi - lt;
+        if (units - unit > stride) next_len = p.lens[(unit + stride) / per_request];
+    };
+    if constexpr (ALONE) {
+        if (unit >= units) return;
+        begin_unit(p.lens[unit / per_request]);
+    } else     if (p.cluster > 0) {
+        const int rank = static_cast<int>(cluster_rank()), mine = share / p.cluster;
+        lb = mine / per_request;
+        lu = mine - lb * per_request;
         lr = key_range<C::kTile>(p, p.lens[lb]);
         const int tiles = lr.tile_hi - lr.tile_lo;       // 8 CTAs at most, of ten tiles
         lt = lr.tile_lo + tiles * rank / p.cluster;
@@ -804,10 +821,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     } else {
         long long total, begin, at;                  // places: all of them, the share's first, the request's first
         int len;
-        const long long units = static_cast<long long>(p.batch) * per_request;
         auto count = [&](long long tiles) {          // the share, now that the number of tiles is known
             gap = tiles >= static_cast<long long>(kLongShare) * gridDim.x ? C::kUnitEnd : 0;
-            total = tiles + gap * units;
+            total = tiles + static_cast<long long>(gap) * units;
             const int shares = total < gridDim.x ? static_cast<int>(total) : static_cast<int>(gridDim.x);
             if (share >= shares) return false;       // fewer tiles than CTAs, so the cuts are told by unit
             begin = share_begin(share, total, shares);
@@ -922,7 +938,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     int page = 0, row_in = 0;
     bool found = false;
     auto look_up = [&]() {
-        const int key = lt * C::kTile + warp * KEYS + (lane % KEYS);
+        const int key = lt * TILE + (ALONE ? 0 : warp * KEYS) + (lane % KEYS);
         found = key >= lr.lo && key < lr.hi;
         if (found) {
             const int at = page_of(key, p.page);
@@ -932,7 +948,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
     };
     look_up();
 
-    if (left == 0) {                                 // a cluster that has more CTAs than the unit tiles
+    if (!ALONE && left == 0) {                       // a cluster that has more CTAs than the unit tiles
         for (int r = tid; r < ROWS; r += kAttnThreads)
             *reinterpret_cast<float2*>(s_ring + (ROWS * D + 2 * r) * 4) = make_float2(-INFINITY, 0.f);
         join_cluster<D, BF16, ROWS>(p, reinterpret_cast<const float*>(s_ring));
@@ -966,21 +982,31 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
                 Step& st = s_step[warp][load_stage];
                 st.b = lb;
                 st.unit = lu;
-                st.rel = lt * C::kTile + warp * KEYS - (lr.hi - 1);
+                st.rel = lt * TILE + (ALONE ? 0 : warp * KEYS) - (lr.hi - 1);
                 st.mask = KEYS == 32 ? mask : mask & 0xffffu;
-                st.last = (left <= (lt + 1 == lr.tile_hi ? 1 + gap : 1) ? 1 : 0) | (lt + 1 == lr.tile_hi ? 2 : 0);
+                if constexpr (ALONE) st.last = left > 1 ? 0 : units - unit > stride ? 2 : 3;
+                else st.last = (left <= (lt + 1 == lr.tile_hi ? 1 + gap : 1) ? 1 : 0) | (lt + 1 == lr.tile_hi ? 2 : 0);
             }
-            left -= lt + 1 == lr.tile_hi ? 1 + gap : 1;
-            if (left > 0) {
-                if (++lt == lr.tile_hi) {
-                    if (++lu == per_request) {
-                        lu = 0;
-                        ++lb;
-                        lr = key_range<C::kTile>(p, p.lens[lb]);
-                    }
-                    lt = lr.tile_lo;
+            if constexpr (ALONE) {
+                ++lt;
+                if (--left == 0 && units - unit > stride) {
+                    unit += stride;
+                    begin_unit(next_len);
                 }
-                look_up();
+                if (left > 0) look_up();
+            } else {
+                left -= lt + 1 == lr.tile_hi ? 1 + gap : 1;
+                if (left > 0) {
+                    if (++lt == lr.tile_hi) {
+                        if (++lu == per_request) {
+                            lu = 0;
+                            ++lb;
+                            lr = key_range<C::kTile>(p, p.lens[lb]);
+                        }
+                        lt = lr.tile_lo;
+                    }
+                    look_up();
+                }
             }
         }
         cp_async_commit();
@@ -1151,6 +1177,33 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         if (st.last == 0) continue;
 
+        if constexpr (ALONE) {
+            // ---- the unit ends: this warp has all of it
+            if ((st.last & 1) == 0) {
+                const Step& next = s_step[warp][stage];
+                ask_queries(next.b, next.unit);
+            }
+            const long long head0 = static_cast<long long>(st.b) * p.heads + hk * p.group;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float x = l[0][r];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                const int row = (lane % 4) * 2 + r;
+                if (row >= p.group) continue;
+                const float inv = x == 0.f ? 0.f : 1.f / x;
+                uint16_t* const out = p.out + (head0 + row) * D + lane / 4;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) out[t * 16 + h * 8] = static_cast<uint16_t>(pack2<BF16>(o[t][0][r + 2 * h] * inv, 0.f));
+                if (lane < 4) store_lse(p, head0 + row, x, m[0][r]);
+            }
+            if ((st.last & 1) != 0) break;
+            fresh = true;
+            continue;
+        }
         // ---- the unit ends, or the share does: the four warps' results become one.  Each warp scales its own to the
         // maximum of the four; what is left is a sum, eight heads at a time through shared memory.
         if (!C::kQueryInSmem && (st.last & 1) == 0) {
@@ -1234,7 +1287,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kCtas) paged_att
         from_begin = true;
     }
     cp_async_wait<0>();
-    if (p.cluster > 1) join_cluster<D, BF16, ROWS>(p, reinterpret_cast<const float*>(s_ring));
+    if (!ALONE && p.cluster > 1) join_cluster<D, BF16, ROWS>(p, reinterpret_cast<const float*>(s_ring));
 }
 
 // Joins the parts of the units that several shares worked on.  CTA (x, y): the unit of cut x, rows from
@@ -1463,10 +1516,17 @@ static int launch_rotary(const RotaryParams& p, bool interleaved, long long toke
 // and 15.5; 16 of 2000 (8) 14.8 and 16.1, of 3000 (12) 19.4 and 19.0.
 constexpr int kUnitTiles = 4, kUnitTilesFull = 6;
 constexpr int kMostCluster = 8;
+// Many short units: one warp each, nothing to join (up to 8 heads; more keep four warps busy at the end of a unit as
+// well).  Up to so many keys, and in proportion fewer where there are fewer units than 3 per CTA, three quarters of the
+// warps.  Against equal shares, 32 KV heads of 128: 128 requests of up to 30 keys 13.5 and 46.6 us, of 200 50.7 and 60.7,
+// of 400 94.4 and 91.5; 32 requests of 400 29.4 and 30.0; 16 requests (512 units) of 200 14.9 and 15.0, of 400 26.4 and
+// 20.0.  At 64: 128 requests of 30 7.2 and 29.5, of 400 48.5 and 49.8, of 700 80.9 and 78.8.
+constexpr int kAloneKeys = 384, kAloneUnits = 3;
 
 struct AttnPlan {
     int grid, nt, row_blocks;
     int cluster;
+    bool alone;
     long long part_floats;
     int cuts, rows_per_cta, join_warps;       // of the joining kernel
     size_t cut_bytes, bytes;
@@ -1518,6 +1578,14 @@ static int make_attn_plan(const FaPagedAttentionArgs* a, int sms, AttnPlan* plan
     const long long seen = a->window > 0 && a->window < capacity ? a->window / attn_tile(D) + 2 : tiles;      // of one unit, at most
     int cluster = 1;
     while (cluster < kMostCluster && 2 * cluster <= seen && 2 * cluster * units <= resident) cluster *= 2;
+    const long long most_keys = a->window > 0 && a->window < capacity ? a->window : capacity;
+    if (plan->nt == 1 && units > resident &&
+        most_keys * kAloneUnits * resident <= kAloneKeys * (units < kAloneUnits * resident ? units : kAloneUnits * resident)) {
+        plan->alone = true;
+        plan->cluster = 1;                             // (nothing is cut)
+        plan->grid = static_cast<int>((units + kWarps - 1) / kWarps < resident ? (units + kWarps - 1) / kWarps : resident);
+        return FA_PAGED_OK;
+    }
     const long long ctas = units * cluster;
     if (seen <= 1 || (ctas <= resident && seen <= cluster * (kUnitTiles + kUnitTilesFull * ctas / resident))) {
         plan->cluster = cluster;
@@ -1555,13 +1623,13 @@ static int attn_plan(const FaPagedAttentionArgs* a, AttnPlan* plan) {
     return a->cache.head_dim == 128 ? make_attn_plan<128>(a, sms, plan) : make_attn_plan<64>(a, sms, plan);
 }
 
-template <int D, bool BF16, int NT, bool CAP>
+template <int D, bool BF16, int NT, bool CAP, bool ALONE>
 static int launch_attention(const AttnParams& p, const AttnPlan& plan, int device, cudaStream_t stream) {
     static std::atomic<unsigned long long> done{0};
     constexpr int smem = AttnCfg<D, NT>::kSmem;
-    int rc = allow_smem(paged_attention_kernel<D, BF16, NT, CAP>, smem, done, device);
+    int rc = allow_smem(paged_attention_kernel<D, BF16, NT, CAP, ALONE>, smem, done, device);
     if (rc != FA_PAGED_OK) return rc;
-    rc = launch_cluster(paged_attention_kernel<D, BF16, NT, CAP>, dim3(plan.grid), kAttnThreads, smem, plan.cluster, stream, p);
+    rc = launch_cluster(paged_attention_kernel<D, BF16, NT, CAP, ALONE>, dim3(plan.grid), kAttnThreads, smem, plan.cluster, stream, p);
     if (rc != FA_PAGED_OK || plan.cluster > 0) return rc;
     const int rows = p.group < NT * 8 ? p.group : NT * 8;
     const dim3 grid(plan.cuts, (rows + plan.rows_per_cta - 1) / plan.rows_per_cta);
@@ -1570,8 +1638,13 @@ static int launch_attention(const AttnParams& p, const AttnPlan& plan, int devic
 
 template <int D, bool BF16, int NT>
 static int launch_attention(const AttnParams& p, const AttnPlan& plan, bool cap, int device, cudaStream_t stream) {
-    return cap ? launch_attention<D, BF16, NT, true>(p, plan, device, stream)
-               : launch_attention<D, BF16, NT, false>(p, plan, device, stream);
+    if constexpr (NT == 1) {
+        if (plan.alone)
+            return cap ? launch_attention<D, BF16, NT, true, true>(p, plan, device, stream)
+                       : launch_attention<D, BF16, NT, false, true>(p, plan, device, stream);
+    }
+    return cap ? launch_attention<D, BF16, NT, true, false>(p, plan, device, stream)
+               : launch_attention<D, BF16, NT, false, false>(p, plan, device, stream);
 }
 
 template <int D, bool BF16>

@@ -157,6 +157,21 @@ def test_attention_split_over_the_gpu(B, H, Hk, d, length):
         assert torch.equal(ops.paged_attention(*args), got)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("H,Hk,B", [(16, 16, 28), (32, 32, 17), (40, 5, 120), (6, 2, 300), (21, 7, 75)])
+def test_attention_of_many_short_requests(d, H, Hk, B):
+    """More units than CTAs: one warp each, or shares with many ends of units."""
+    r = random.Random(B)
+    slopes = (2.0 ** (-8.0 * torch.arange(1, H + 1) / H)).float().cuda()
+    for most in (1, 20, 350):
+        lens = [r.choice((0, 1, 17, most, r.randint(0, most))) for _ in range(B)]
+        args = make_cache(lens, H=H, Hk=Hk, d=d, page_size=24, dtype=DTYPES[most % 2], gen=gen(most), fill=float("nan"))
+        attend_and_check(*args, what=f"up to {most}")
+        attend_and_check(*args, what=f"up to {most}, all of it", window=19, softcap=20.0, slopes=slopes)
+    args = make_cache([1000 if b % 9 == 0 else 130 for b in range(B)], H=H, Hk=Hk, d=d, page_size=64, dtype=torch.float16, gen=gen(B))
+    attend_and_check(*args, what="a window", window=100)
+
+
 @pytest.mark.parametrize("d,H,Hk", [(128, 8, 2), (64, 4, 4), (128, 32, 1)])
 def test_attention_of_one_long_among_many_short(d, H, Hk):
     """Shares that hold hundreds of ends of units, and a unit that is cut in most of the parts."""

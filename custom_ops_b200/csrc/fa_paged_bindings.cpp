@@ -197,6 +197,7 @@ void paged_shrink_(const Tensor& block_table, const Tensor& seq_lens, const Tens
                    const Tensor& free_head, int64_t page_size) {
     const char* op = "paged_shrink_";
     check_table(block_table, seq_lens, keep_lens, free_pages, free_head, page_size, op);
+    at::assert_no_partial_overlap(seq_lens, keep_lens);
     const c10::cuda::CUDAGuard guard(block_table.device());
     FaPagedShrinkArgs a{};
     a.struct_size = sizeof(a);
@@ -266,6 +267,10 @@ FaPagedAppendArgs append_args(const Tensor& k, const Tensor& v, const Tensor& sl
     check_rows(k, op, "k");
     check_rows(v, op, "v");
     check_list(slots, k.size(0), true, op, "slots");
+    for (const Tensor* t : {&k, &v}) {        // rows would be read while others are written
+        at::assert_no_overlap(k_cache, *t);
+        at::assert_no_overlap(v_cache, *t);
+    }
     a.struct_size = sizeof(a);
     a.device = k.get_device();
     a.k = k.data_ptr();
@@ -286,6 +291,8 @@ Tensor rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Te
     TORCH_CHECK(q.dtype() == k.dtype(), op, ": q dtype must match k");
     TORCH_CHECK(q.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2), op, ": q must be 3D (T, H, d)");
     check_rows(q, op, "q");
+    at::assert_no_overlap(k_cache, q);
+    at::assert_no_overlap(v_cache, q);
     check_list(positions, k.size(0), true, op, "positions");
     a.rotary = rotary_of(positions, freqs, interleaved, mscale, false, q.size(2), op);
     const c10::cuda::CUDAGuard guard(q.device());

@@ -576,6 +576,25 @@ def test_append_refusals():
     ops.paged_append(x[:0], x[:0], s[:0], c, c2)
 
 
+def test_operands_inside_what_is_written_are_refused():
+    c, c2 = (torch.zeros(4, 2, 8, 64, device="cuda").half() for _ in range(2))
+    x, s = torch.zeros(3, 2, 64, device="cuda").half(), torch.zeros(3, dtype=torch.int64, device="cuda")
+    freqs, _ = rotary_frequencies(64, 10000.0)
+    for inside in (c.view(-1, 2, 64)[4:7], c2.view(-1, 2, 64)[:3]):
+        for k, v in ((inside, x), (x, inside)):
+            with pytest.raises(RuntimeError, match="memory location"):
+                ops.paged_append(k, v, s, c, c2)
+        with pytest.raises(RuntimeError, match="memory location"):
+            ops.rotary_append(inside, x, x, s, s, c, c2, freqs)
+    lens = torch.full((9,), 5, dtype=torch.int32, device="cuda")
+    table, free = torch.zeros(8, 2, dtype=torch.int32, device="cuda"), torch.arange(16, dtype=torch.int32, device="cuda")
+    head = torch.full((1,), 16, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="memory location"):
+        ops.paged_shrink_(table, lens[:8], lens[1:], free, head, 4)
+    ops.paged_shrink_(table, lens[:8], lens[:8], free, head, 4)          # one tensor: nothing changes
+    assert (lens == 5).all() and head.item() == 16
+
+
 # ------------------------------------------------------------------ together
 def layered_reference(tokens_q, tokens_k, tokens_v, freqs, mscale, upto):
     """Attention of the token at `upto - 1` of one request over its first `upto` tokens, in 64 bits, from the

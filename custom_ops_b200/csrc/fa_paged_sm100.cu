@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_shrink_kernel(const Shrin
 // are worked out.  Tokens per CTA: as many as keep a thread at kRotaryBatch heads at most, so that all of a CTA's
 // loads are in flight together - unless that leaves SMs without a CTA.  Bound by memory: 4 x 2048 tokens with 16 + 4
 // heads of 128 take 15.6 to 16.9 us, 5.0 to 5.4 TB/s of 6.5 both ways; 8100 tokens with 32 + 8 + 8 heads into the pages
-// 37.4 us, 5.3 TB/s; 64 tokens 7.1 us a call, the host's time.  Measured and left: four heads a thread (fewer CTAs,
+// 37.9 us, 5.3 TB/s; 64 tokens 7.1 us a call, the host's time.  Measured and left: four heads a thread (fewer CTAs,
 // 17.2 us), CTAs that stay and load pieces ahead by cp.async (19.9), loads through shared memory (16.4).
 constexpr int kRotaryThreads = 128;
 constexpr int kRotaryBatch = 3;
@@ -639,11 +639,11 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
 // Precision: a weight p is the sum of two 16-bit numbers (hi + lo), two products instead of one; a single
 // 16-bit weight would add as much error as the rounding of the output.  Sums take the fp32 weight.
 //
-// Measured (calls back to back; memory's rate is 6.54 TB/s): one request of 131072 keys, 32 + 8 heads of 128: 88.4 us,
-// 6.07 TB/s; 32 requests of up to 4096: 61.5, 5.8 TB/s; 48 requests of a window of 1024, 16 heads of 64, capped: 38.2,
-// 5.2 TB/s; 8 requests of up to 7001 with a bias: 22.0, 3.7 TB/s; one of 333: 7.2, the host's time.  Of what is above
+// Measured (calls back to back; memory's rate is 6.54 TB/s): one request of 131072 keys, 32 + 8 heads of 128: 89 us,
+// 6.03 TB/s; 32 requests of up to 4096: 62.0, 5.7 TB/s; 48 requests of a window of 1024, 16 heads of 64, capped: 38.2,
+// 5.2 TB/s; 8 requests of up to 7001 with a bias: 21.2, 3.9 TB/s; one of 333: 7.1, the host's time.  Of what is above
 // the bytes' time, 2 us are the launch and the way to the first load, 2 the first loads' latency, 1.3 the end of a
-// unit, 3 to 4 the joining kernel.  32 heads on one key head: 37 against 14 for the bytes - eight warps an SM with 96
+// unit, 3 to 4 the joining kernel.  32 heads on one key head: 34 against 14 for the bytes - eight warps an SM with 96
 // products a step each do not hide their latencies.
 // Measured and left: warps that share a tile and exchange P, so that accumulators are small (two barriers a tile: 109
 // us for the 131072 keys); bulk copies of a row per lane (issued one by one, 137); joining by the last CTA to

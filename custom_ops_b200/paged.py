@@ -33,10 +33,13 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional
     ``scaling`` stretches them for contexts ``factor`` times longer than a model was trained on:
     ``"linear"``   all angles divided by ``factor``;
     ``"base"``     the base raised to ``base * factor ** (rot_dim / (rot_dim - 2))``: the slowest pair is divided by
-                   ``factor``, the fastest stays;
-    ``"by_parts"`` pairs that turn more than ``fast`` times within ``original_length`` positions stay, those that
-                   turn less than ``slow`` times are divided by ``factor``, linearly in between by the pair's
-                   index; ``mscale`` is ``0.1 * log(factor) + 1``.
+                   ``factor``, the fastest stays (published as "NTK-aware" scaling);
+    ``"by_parts"`` pairs that turn at least ``fast`` times within ``original_length`` positions stay, those that
+                   turn at most ``slow`` times are divided by ``factor``, linearly in between by the pair's
+                   index, from the last that turns ``fast`` times to the first that turns no more than ``slow``
+                   times, also where these lie outside the head's pairs; ``mscale`` is ``0.1 * log(factor) + 1``
+                   ("NTK-by-parts" with YaRN's factor; Peng et al., 2023, arXiv:2309.00071.  Forms of it that move
+                   the ends of the ramp onto the head's first and last pair differ where these would lie outside).
     """
     if rot_dim < 2 or rot_dim % 2 != 0:
         raise ValueError("rot_dim must be even and at least 2")
@@ -60,9 +63,8 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional
         def pair_that_turns(times):          # its (fractional) index
             return rot_dim * math.log(original_length / (times * 2 * math.pi)) / (2 * math.log(base))
 
-        lo = max(0.0, math.floor(pair_that_turns(fast)))
-        hi = min(rot_dim // 2 - 1.0, math.ceil(pair_that_turns(slow)))
-        ramp = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+        lo, hi = math.floor(pair_that_turns(fast)), math.ceil(pair_that_turns(slow))
+        ramp = ((i / 2 - lo) / max(hi - lo, 1)).clamp(0.0, 1.0)
         freqs = freqs * (1.0 - ramp) + freqs / factor * ramp
         mscale = 0.1 * math.log(factor) + 1.0
     return freqs.to(device if device is not None else "cuda"), mscale

@@ -207,6 +207,7 @@ int fa_paged_append_sm100(const FaPagedAppendArgs* args, void* stream);
  * cache are hidden; what the cache holds behind a request's length or ahead of its window is never used, and
  * only pages with a visible key are looked up.
  * Weights, sums and accumulators are fp32 (a weight enters the product with v as the sum of two 16-bit numbers).
+ * The cap adds an error of at most cap * 2^-21 to a score up to a cap of 64, of 2^-18.9 of the score above that.
  * Long histories are split over the GPU and joined through the workspace; the result depends, within the fp32
  * rounding of the join, on the number of SMs, never on timing.
  */

@@ -109,6 +109,28 @@ def usual_slopes(H):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,H,Hk", [(128, 12, 4), (64, 12, 1), (128, 32, 1), (64, 8, 8)])
+@pytest.mark.parametrize("window", [0, 65, 200])
+def test_biased_scores_key_by_key(dtype, d, H, Hk, window):
+    args = make_cache([1, 64, 130, 1500, 0, 4099], H=H, Hk=Hk, d=d, page_size=24, dtype=dtype, gen=torch.Generator().manual_seed(3))
+    check(args, "usual", window=window, slopes=usual_slopes(H), scale=0.11)
+    check(args, "usual, capped", window=window, slopes=usual_slopes(H), scale=0.11, softcap=5.0)
+    mixed = usual_slopes(H)                              # some heads without a bias, one towards the oldest key
+    mixed[::3], mixed[1] = 0.0, -0.01
+    check(args, "mixed", window=window, slopes=mixed, scale=0.11)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_steep_biases_key_by_key(dtype):
+    args = make_cache([700, 1, 90, 20000], H=4, Hk=2, d=64, page_size=16, dtype=dtype, gen=torch.Generator().manual_seed(8))
+    for slope in (100.0, 1.0, 0.05):
+        check(args, f"slope {slope}", slopes=torch.full((4,), slope, device="cuda"))
+    args = make_cache([700, 1, 90, 300], H=4, Hk=2, d=64, page_size=16, dtype=dtype, gen=torch.Generator().manual_seed(8))
+    for slope in (-5.0, -0.2):                           # towards the oldest key, whose bias is the largest number
+        check(args, f"slope {slope}", slopes=torch.full((4,), slope, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d,H,Hk", [(128, 8, 2), (64, 16, 1), (64, 32, 1)])
 @pytest.mark.parametrize("cap", [20.0, 64.0, 80.0, 1e3, 1e4, 1e6, 1e7, 1e30])
 def test_capped_scores_key_by_key(dtype, d, H, Hk, cap):

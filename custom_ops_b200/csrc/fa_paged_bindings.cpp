@@ -15,6 +15,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <limits>
 
@@ -238,17 +239,22 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor
     auto q_out = empty({B, H, S, d}, q.scalar_type(), q), k_out = empty({B, Hk, S, d}, q.scalar_type(), q);
     a.struct_size = sizeof(a);
     a.device = q.get_device();
-    a.q = q.data_ptr();
-    a.k = k.data_ptr();
-    a.q_out = q_out.data_ptr();
-    a.k_out = k_out.data_ptr();
     a.q_batch_stride = step(q, 0), a.q_head_stride = step(q, 1), a.q_row_stride = step(q, 2);
     a.k_batch_stride = step(k, 0), a.k_head_stride = step(k, 1), a.k_row_stride = step(k, 2);
     a.position_batch_stride = positions.dim() == 2 ? step(positions, 0) : 0;
-    a.batch = as_i32(B, "the batch"), a.heads = as_i32(H, "the number of heads");
+    a.heads = as_i32(H, "the number of heads");
     a.heads_k = as_i32(Hk, "the number of key heads"), a.seqlen = as_i32(S, "the length");
     a.head_dim = static_cast<int32_t>(d);
-    check_rc(fa_rotary_sm100(&a, stream_of(q)), op);
+    const auto at = [](const Tensor& t, int64_t elements) { return static_cast<char*>(t.data_ptr()) + elements * t.element_size(); };
+    for (int64_t b = 0; b < B; b += FA_ROTARY_MAX_BATCH) {
+        a.batch = static_cast<int32_t>(std::min<int64_t>(B - b, FA_ROTARY_MAX_BATCH));
+        a.q = at(q, b * a.q_batch_stride);
+        a.k = at(k, b * a.k_batch_stride);
+        a.q_out = at(q_out, b * H * S * d);
+        a.k_out = at(k_out, b * Hk * S * d);
+        a.rotary.positions = at(positions, b * a.position_batch_stride);
+        check_rc(fa_rotary_sm100(&a, stream_of(q)), op);
+    }
     return {q_out, k_out};
 }
 

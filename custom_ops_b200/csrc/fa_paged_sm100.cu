@@ -1736,7 +1736,7 @@ static int rotary(const FaRotaryArgs* a, cudaStream_t stream) {
     if (a->batch < 0 || a->heads < 0 || a->heads_k < 0 || a->seqlen < 0 || a->position_batch_stride < 0)
         return FA_PAGED_ERR_SHAPE;
     if (a->head_dim != 64 && a->head_dim != 128) return FA_PAGED_ERR_HEAD_DIM;
-    if (a->batch > 65535 || static_cast<long long>(a->heads) + a->heads_k > (1 << 24)) return FA_PAGED_ERR_SHAPE;
+    if (a->batch > FA_ROTARY_MAX_BATCH || static_cast<long long>(a->heads) + a->heads_k > (1 << 24)) return FA_PAGED_ERR_SHAPE;
     if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->q_out) || !aligned16(a->k_out) || !stride8(a->q_batch_stride) ||
         !stride8(a->q_head_stride) || !stride8(a->q_row_stride) || !stride8(a->k_batch_stride) || !stride8(a->k_head_stride) ||
         !stride8(a->k_row_stride))

@@ -149,8 +149,10 @@ typedef struct FaRotarySpec {
 /*
  * q (batch, heads, seqlen, head_dim), k (batch, heads_k, seqlen, head_dim) through their strides ->
  * q_out, k_out contiguous.  positions[b * position_batch_stride + s].  heads_k may be 0.
- * An output must not overlap an input.
+ * An output must not overlap an input.  At most FA_ROTARY_MAX_BATCH batch rows a call (a grid's second dimension);
+ * the torch operator takes more in several launches.
  */
+#define FA_ROTARY_MAX_BATCH 65535
 typedef struct FaRotaryArgs {
     uint32_t struct_size;
     int32_t device;

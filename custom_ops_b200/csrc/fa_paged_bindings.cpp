@@ -53,10 +53,11 @@ int32_t dtype_code(const Tensor& q, const char* op) {
     return q.dtype() == torch::kBFloat16 ? FA_PAGED_BF16 : FA_PAGED_FP16;
 }
 
-// Stride of a dimension; that of a dimension of one element says nothing.
-int64_t step(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+// Stride of a dimension; that of a dimension of one element says nothing, nor do those of a tensor without any.
+int64_t step(const Tensor& t, int64_t dim) { return t.size(dim) > 1 && t.numel() > 0 ? t.stride(dim) : 0; }
 
 void check_rows(const Tensor& t, const char* op, const char* name) {
+    if (t.numel() == 0) return;
     TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, op, ": the last dimension of ", name, " must be contiguous");
     TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, op, ": ", name, " must be 16-byte aligned");
     for (int64_t i = 0; i + 1 < t.dim(); ++i)
@@ -258,6 +259,57 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor
     return {q_out, k_out};
 }
 
+// Recorded gradients: the rotation is linear, so the gradient is one call of the operator, turning the other way.
+using RotaryCall = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, bool, double, bool);
+
+const c10::TypedOperatorHandle<RotaryCall>& rotary_op() {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("recsys_ops::rotary", "").typed<RotaryCall>();
+    return op;
+}
+
+// A gradient may come in any layout; the operator wants whole rows, 16-byte aligned.
+Tensor as_rows(const Tensor& t) {
+    const Tensor c = t.contiguous();
+    return c.sym_storage_offset() % 8 == 0 ? c : c.clone();
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                                                  const Tensor& positions, const Tensor& freqs, bool interleaved, double mscale,
+                                                  bool adjoint) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({positions, freqs});
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["mscale"] = mscale;
+        ctx->saved_data["adjoint"] = adjoint;
+        auto [q_out, k_out] = rotary_op().call(q, k, positions, freqs, interleaved, mscale, adjoint);
+        return {q_out, k_out};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        // heads whose gradient nobody wants are left out
+        const bool for_q = ctx->needs_input_grad(0), for_k = ctx->needs_input_grad(1);
+        const Tensor dq = as_rows(for_q ? grads[0] : grads[0].narrow(1, 0, 0));
+        const Tensor dk = as_rows(for_k ? grads[1] : grads[1].narrow(1, 0, 0));
+        auto [gq, gk] = rotary_op().call(dq, dk, saved[0], saved[1], ctx->saved_data["interleaved"].toBool(),
+                                         ctx->saved_data["mscale"].toDouble(), !ctx->saved_data["adjoint"].toBool());
+        return {for_q ? gq : Tensor(), for_k ? gk : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+std::tuple<Tensor, Tensor> rotary_autograd(c10::DispatchKeySet keys, const Tensor& q, const Tensor& k, const Tensor& positions,
+                                           const Tensor& freqs, bool interleaved, double mscale, bool adjoint) {
+    if (c10::GradMode::is_enabled()) {
+        TORCH_CHECK(!freqs.requires_grad(), "rotary: no gradient is recorded for freqs");
+        if (q.requires_grad() || k.requires_grad()) {
+            auto out = RotaryFunction::apply(q, k, positions, freqs, interleaved, mscale, adjoint);
+            return {out[0], out[1]};
+        }
+    }
+    return rotary_op().redispatch(keys & c10::after_ADInplaceOrView_keyset, q, k, positions, freqs, interleaved, mscale, adjoint);
+}
+
 FaPagedAppendArgs append_args(const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor& k_cache,
                               const Tensor& v_cache, const char* op) {
     FaPagedAppendArgs a{};
@@ -420,5 +472,7 @@ TORCH_LIBRARY_IMPL(recsys_ops, CompositeExplicitAutograd, m) {
     m.impl("paged_attention", &paged_attention);
     m.impl("paged_attention_lse", &paged_attention_lse);
 }
+
+TORCH_LIBRARY_IMPL(recsys_ops, Autograd, m) { m.impl("rotary", &rotary_autograd); }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) { m.doc() = "recsys_ops / paged group: paged key/value cache for sm_100a"; }

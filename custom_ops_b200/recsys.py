@@ -646,8 +646,9 @@ class RecsysOps:
 
         ``positions`` int32 or int64 ``(S,)`` or ``(B, S)``; ``freqs`` float64, one angle per position and pair
         (``paged.rotary_frequencies``): ``2 * len(freqs)`` elements of each head turn, in pairs ``(i, i + n)``
-        or, ``interleaved``, ``(2i, 2i + 1)``; the rest pass through.  Pairs are scaled by ``mscale``.  Nothing
-        here records gradients; ``adjoint`` turns the other way, which is the gradient with respect to q and k."""
+        or, ``interleaved``, ``(2i, 2i + 1)``; the rest pass through.  Pairs are scaled by ``mscale``.
+        ``adjoint`` turns the other way, which is the gradient with respect to q and k; it is recorded where q or k
+        wants one (``freqs`` must not).  No other operator of this group records gradients."""
         return self._paged_call(backend, "rotary")(q, k, positions, freqs, interleaved, mscale, adjoint)
 
     def rotary_append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,

@@ -118,6 +118,20 @@ FaRotarySpec rotary_of(const Tensor& positions, const Tensor& freqs, bool interl
 }
 
 // ------------------------------------------------------------------ tables
+// Two contiguous tensors must not share memory.
+void check_apart(const Tensor& a, const Tensor& b, const char* op) {
+    const char *x = static_cast<const char*>(a.data_ptr()), *y = static_cast<const char*>(b.data_ptr());
+    TORCH_CHECK(x + a.nbytes() <= y || y + b.nbytes() <= x, op, ": a tensor that is written shares a memory location with another");
+}
+
+// What a call updates in place, or reads while it does.  (The lengths to add or to keep are read before anything is
+// written; they may be the lengths themselves.)
+void check_in_place(const Tensor& seq_lens, const Tensor& free_pages, const Tensor& free_head, const char* op) {
+    check_apart(seq_lens, free_pages, op);
+    check_apart(seq_lens, free_head, op);
+    check_apart(free_pages, free_head, op);
+}
+
 void check_table(const Tensor& block_table, const Tensor& seq_lens, const Tensor& other, const Tensor& free_pages,
                  const Tensor& free_head, int64_t page_size, const char* op) {
     check_cuda(op, {&block_table, &seq_lens, &other, &free_pages, &free_head});
@@ -129,6 +143,8 @@ void check_table(const Tensor& block_table, const Tensor& seq_lens, const Tensor
     check_list(other, B, false, op, "new_lens or keep_lens");
     check_list(free_pages, free_pages.numel(), false, op, "free_pages");
     check_list(free_head, 1, false, op, "free_head");
+    if (block_table.is_contiguous())
+        for (const Tensor* t : {&seq_lens, &other, &free_pages, &free_head}) check_apart(block_table, *t, op);
     TORCH_CHECK(page_size > 0, op, ": page_size must be positive");
     TORCH_CHECK(page_size <= std::numeric_limits<int32_t>::max() &&
                     block_table.size(1) <= std::numeric_limits<int32_t>::max() / page_size,
@@ -190,6 +206,7 @@ std::tuple<Tensor, Tensor, Tensor> paged_extend_(const Tensor& block_table, cons
     const char* op = "paged_extend_";
     check_table(block_table, seq_lens, new_lens, free_pages, free_head, page_size, op);
     check_num_tokens(num_tokens, op);
+    check_in_place(seq_lens, free_pages, free_head, op);
     const c10::cuda::CUDAGuard guard(block_table.device());
     auto r = extend(block_table, seq_lens, new_lens, free_pages, free_head, page_size, num_tokens, seq_lens, free_head, op);
     return {r.slots, r.positions, r.cu};
@@ -200,6 +217,7 @@ void paged_shrink_(const Tensor& block_table, const Tensor& seq_lens, const Tens
     const char* op = "paged_shrink_";
     check_table(block_table, seq_lens, keep_lens, free_pages, free_head, page_size, op);
     at::assert_no_partial_overlap(seq_lens, keep_lens);
+    check_in_place(seq_lens, free_pages, free_head, op);
     const c10::cuda::CUDAGuard guard(block_table.device());
     FaPagedShrinkArgs a{};
     a.struct_size = sizeof(a);

@@ -30,7 +30,8 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 }
 // Lets the next kernel of the stream become resident / waits until the kernel before has finished.  The rotary
 // and attention kernels do not announce the next one early: resident CTAs of the next take their places SM by SM as theirs
-// leave, which spread the next call unevenly (48 requests, 16 heads of 64: 53 us a call with it, 40 without).
+// leave, which spread the next call unevenly (48 requests, 16 heads of 64, an earlier form of the kernel: 53 us a call
+// with it, 40 without).
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -632,9 +633,9 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
 // Products: with few query rows the keys are the rows of the mma: S^T (16 keys x 8 heads) = K Q^T and
 // O^T (16 of d x 8 heads) += V^T P^T.  Eight heads to a tile waste half of what sixteen would, and the
 // accumulators are half as many.  K and V come through ldmatrix (V transposed); P^T moves from the accumulator
-// layout to the operand's by movmatrix.  mma.sync is enough here: at 8 heads a tile the tensor pipe is busy for
-// about a tenth of the time the loads take, and tcgen05's 128-row tiles would be filled with 8 rows or would
-// need P^T in shared memory.
+// layout to the operand's by movmatrix.  mma.sync is enough up to 8 heads a tile: the tensor pipe is busy for 15 % of
+// the time, and tcgen05, with 128 keys as its rows, would want P^T in shared memory.  With 16 and 32 heads it is not:
+// registers leave room for eight warps an SM, too few to hide the products' latencies.
 //
 // Precision: a weight p is the sum of two 16-bit numbers (hi + lo), two products instead of one; a single
 // 16-bit weight would add as much error as the rounding of the output.  Sums take the fp32 weight.
@@ -666,7 +667,8 @@ struct AttnCfg {
     static constexpr int kTile = kKeys * kWarps;
     static constexpr int kStageBytes = kKeys * D * 2 * 2;
     // Stages and CTAs per SM: what shared memory and registers allow.  24 to 32 KB in flight per warp and three stages
-    // read 6.4 of 6.5 TB/s; at 64, more warps hide the softmax, twice the work per byte (35 us against 77 with two CTAs).
+    // read 6.0 of 6.5 TB/s in the longest call; at 64, more warps hide the softmax, twice the work per byte (35 us against
+    // 77 with two CTAs).
     static constexpr int kStages = NT > 2 || D == 64 ? 2 : 3;
     static constexpr int kCtas = D == 64 && NT == 1 ? 3 : 2;
     static constexpr int kUnitEnd = (NT > 2 ? 2 : 1) * (D == 64 ? 1 : 2);      // tiles that the end of a unit counts as
@@ -1535,7 +1537,9 @@ static int launch_rotary(const RotaryParams& p, bool interleaved, long long toke
                 : launch_rotary<64, false>(p, interleaved, tokens, outer, sms, stream);
 }
 
-// Short units: each is done by a cluster of 1 to 8 CTAs that join their parts through their shared memory.  No sums
+// Short units, as far as the table's width and the window show it (the lengths are on the device; a request of 333 keys
+// takes 5.7 us of GPU time under a table of 368 and 6.3 under one of 8192, called from Python 7 and 9): each is done by a
+// cluster of 1 to 8 CTAs that join their parts through their shared memory.  No sums
 // over the lengths, no partial results in memory, no second kernel (which costs the host 2.7 us, too).  Up to so many
 // tiles for a CTA: 4, and 6 more as the clusters fill the GPU, where equal shares of all keys have no SMs to win.  GPU
 // time with clusters and with equal shares, 4 KV heads of 128: one request of 300 keys 5.9 and 6.5 us, of 2000 (4 tiles
@@ -1544,10 +1548,11 @@ static int launch_rotary(const RotaryParams& p, bool interleaved, long long toke
 constexpr int kUnitTiles = 4, kUnitTilesFull = 6;
 constexpr int kMostCluster = 8;
 // Many short units: one warp each, nothing to join (up to 8 heads; more keep four warps busy at the end of a unit as
-// well).  Up to so many keys, and in proportion fewer where there are fewer units than 3 per CTA, three quarters of the
-// warps.  Against equal shares, 32 KV heads of 128: 128 requests of up to 30 keys 13.5 and 46.6 us, of 200 50.7 and 60.7,
-// of 400 94.4 and 91.5; 32 requests of 400 29.4 and 30.0; 16 requests (512 units) of 200 14.9 and 15.0, of 400 26.4 and
-// 20.0.  At 64: 128 requests of 30 7.2 and 29.5, of 400 48.5 and 49.8, of 700 80.9 and 78.8.
+// well).  Up to so many keys that the table or the window could hold, and in proportion fewer where there are fewer units
+// than 3 per CTA, three quarters of the warps.  Against equal shares, 32 KV heads of 128: 128 requests of up to 30 keys
+// 13.5 and 46.6 us, of 200 50.7 and 60.7, of 400 94.4 and 91.5; 32 requests of 400 29.4 and 30.0; 16 requests (512 units)
+// of 200 14.9 and 15.0, of 400 26.4 and 20.0.  At 64: 128 requests of 30 7.2 and 29.5, of 400 48.5 and 49.8, of 700 80.9
+// and 78.8.
 constexpr int kAloneKeys = 384, kAloneUnits = 3;
 
 struct AttnPlan {

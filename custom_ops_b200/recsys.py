@@ -614,7 +614,7 @@ class RecsysOps:
         those it has.  ``seq_lens``, ``new_lens`` int32 ``(B,)``: tokens held, tokens to add.  ``free_pages``
         int32 ``(F,)`` is taken from index ``free_head`` (int32 ``(1,)``) on, in the order of the requests.
         A request that the table has no columns for, or the list no pages, gets nothing; once the list has run
-        out, neither does any later request that needs a page.
+        out, neither does any later request that needs a page.  At most 16384 requests.
 
         Returns ``(seq_lens, free_head, slots, positions, cu)``: the new lengths (the old ones where refused)
         and head, and for the ``num_tokens`` packed new tokens their slot (int64, ``page * page_size + row``;
@@ -635,7 +635,8 @@ class RecsysOps:
                       free_pages: torch.Tensor, free_head: torch.Tensor, page_size: int,
                       backend: Optional[str] = None) -> None:
         """Shortens every request to at most ``keep_lens`` tokens (0 releases it) and puts the pages behind that
-        back in front of ``free_head``.  ``seq_lens``, ``free_pages`` and ``free_head`` change in place."""
+        back in front of ``free_head``.  ``seq_lens``, ``free_pages`` and ``free_head`` change in place.  No page may
+        stand in the rows of two requests: it would be given back twice."""
         return self._paged_call(backend, "paged_shrink_")(block_table, seq_lens, keep_lens, free_pages, free_head,
                                                               page_size)
 
@@ -676,7 +677,10 @@ class RecsysOps:
         whose key and value are in the cache.  ``scale`` defaults to ``1 / sqrt(d)``; ``softcap > 0`` turns a
         score x into ``softcap * tanh(x / softcap)``; ``slopes`` (fp32, one per head) add
         ``slope * (key - newest key)``; ``window > 0`` hides all but the last ``window`` keys.
-        A request without a key gives 0."""
+        A request without a key gives 0.
+
+        The work is divided by what the table could hold, not by the lengths, which are on the device: short
+        histories are faster with a table that is no wider than they are (``block_table[:, :columns]``)."""
         return self._paged_call(backend, "paged_attention")(q, k_cache, v_cache, block_table, seq_lens, scale,
                                                                 window, softcap, slopes)
 

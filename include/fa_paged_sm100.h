@@ -12,7 +12,8 @@
  * FA_PAGED_ERR_* code, never throws, never synchronises, never allocates; memory belongs to the caller;
  * work is enqueued on the caller's stream, chained to the kernel before it (every kernel waits for that
  * one before it touches memory).  No kernel here waits for another one's memory, so there is no status
- * word.  The first call of an operator on a device loads its kernel: make it outside any stream capture.  Pointers are device pointers on `device`; `struct_size` is sizeof of the struct, checked.
+ * word.  The first call of an operator with given types, shapes and options loads its kernel: make it outside any stream
+ * capture.  Pointers are device pointers on `device`; `struct_size` is sizeof of the struct, checked.
  *
  * The cache: pages of `page_size` tokens, k and v each (num_pages, heads_k, page_size, head_dim) of one
  * 16-bit type, addressed through their element strides (page, head, token); the last dimension is
@@ -109,7 +110,8 @@ int fa_paged_extend_sm100(const FaPagedExtendArgs* args, void* stream);
  * again: the free list is a stack.  Updates lens, free_pages and free_head in place; the block table keeps
  * its (now unused) entries.  A head that would become negative - pages that never came from this list - is
  * refused on the device: the pages of the requests that would not fit stay where they are, and the requests
- * keep their length.
+ * keep their length.  A page belongs to one request: one that the caller has put into two rows (a prefix that two
+ * requests share) would come back twice, and the next extend would give it to two requests.
  */
 typedef struct FaPagedShrinkArgs {
     uint32_t struct_size;
@@ -211,7 +213,10 @@ int fa_paged_append_sm100(const FaPagedAppendArgs* args, void* stream);
  * Weights, sums and accumulators are fp32 (a weight enters the product with v as the sum of two 16-bit numbers).
  * The cap adds an error of at most cap * 2^-21 to a score up to a cap of 64, of 2^-18.9 of the score above that.
  * Long histories are split over the GPU and joined through the workspace; the result depends, within the fp32
- * rounding of the join, on the number of SMs, never on timing.
+ * rounding of the join, on how they are split - on the number of SMs, the table's width and the lengths of the other
+ * requests of the call - never on timing.  How the work is divided goes by what the table and the window could hold,
+ * since the lengths are on the device: a table no wider than the longest request lets short ones be done in one launch.
+ * An infinite value that a row sees gives NaN (its weight's second part is 0 or negative).
  */
 typedef struct FaPagedAttentionArgs {
     uint32_t struct_size;
